@@ -36,6 +36,13 @@ SIGNATURES = {
     "btm_int4_quantize": (_i, [_i, _vp, _i, _i, _i, _vp, _vp, _vp]),
     "btm_convert": (_i, [_i, _vp, _i, _i, _i64, _vp, _vp]),
     "btm_int4_unpack": (_i, [_i, _vp, _i, _i, _vp, _vp]),
+    "btm_gemm_grouped": (_i, [_i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i64, _vp, _i64, _i64, _i, _vp, _i64]),
+    "btm_gemm_grouped_wgrad": (_i, [_i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64]),
+    "btm_mxfp4_scale_bytes": (_sz, [_i, _i, _i]),
+    "btm_mxfp4_quantize": (_i, [_i, _vp, _i, _i, _i, _i, _vp, _vp, _i64, _vp, _vp]),
+    "btm_mxfp4_dequant": (_i, [_i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i64]),
+    "btm_mxfp4_matmul": (_i, [_i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64]),
+    "btm_mxfp4_matmul_grouped": (_i, [_i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64]),
     "btm_gemm_nshard": (_i, [_i, _vp, _i, _i, _i, _i, _vp, _i64, _vp, _i64, C.POINTER(_vp), _i64, _i, _i]),
     "btm_gemm_nshard_mc": (_i, [_i, _vp, _i, _i, _i, _i, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i]),
     "btm_mc_supported": (_i, [_i]),

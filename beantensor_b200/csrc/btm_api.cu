@@ -396,6 +396,8 @@ int btm_check_device_status(int device, void *stream)
         cudaStreamSynchronize(st);
         if (host == 201)
             return set_error(BTM_ERR_CUDA, "CUDA Error: a debug bounds check stopped a store outside the output (device status %d)", host);
+        if (host == 202)
+            return set_error(BTM_ERR_INVALID, "grouped operator: row offsets decrease or leave the rows (they were clamped; device status %d)", host);
         return set_error(BTM_ERR_TIMEOUT, "CUDA Error: a kernel wait ran out (device status %d)", host);
     }
     return BTM_OK;
@@ -730,6 +732,158 @@ int btm_int4_quantize(int device, void *stream, int N, int K, int group, const v
     DeviceState *ds = device_state(device);
     if (!ds) return last_code();
     return launch_int4_quantize((cudaStream_t)stream, N, K, group, w_f16, out_packed, out_scales_f16);
+}
+
+// Checks that the grouped operators share.
+static int check_groups(const char *what, int groups, int rows, const int32_t *offsets)
+{
+    if (groups < 0 || rows < 0) return set_error(BTM_ERR_INVALID, "%s: negative dimension (groups=%d rows=%d)", what, groups, rows);
+    if (groups > 0 && !offsets) return set_error(BTM_ERR_INVALID, "%s: null offsets", what);
+    if ((uintptr_t)offsets & 3) return set_error(BTM_ERR_INVALID, "%s: offsets are not aligned", what);
+    return BTM_OK;
+}
+
+int btm_gemm_grouped(int device, void *stream, int dtype, int groups, int rows, int N, int K, const int32_t *offsets, const void *A,
+                     int64_t lda, const void *B, int64_t strideB, int64_t ldb, int b_transposed, void *C, int64_t ldc)
+{
+    if (dtype != BTM_F16 && dtype != BTM_BF16)
+        return set_error(BTM_ERR_UNSUPPORTED, "grouped matmul: dtype %d is not supported (Float16, BFloat16 only)", dtype);
+    if (N < 0 || K < 0) return set_error(BTM_ERR_INVALID, "grouped matmul: negative dimension (N=%d K=%d)", N, K);
+    int rc = check_groups("grouped matmul", groups, rows, offsets);
+    if (rc) return rc;
+    if (groups > 0 && rows > 0 && N > 0 && (!C || (K > 0 && (!A || !B)))) return set_error(BTM_ERR_INVALID, "grouped matmul: null pointer");
+    const int64_t b_inner = b_transposed ? K : N, b_outer = b_transposed ? N : K;
+    if (lda < K || ldb < b_inner || ldc < N)
+        return set_error(BTM_ERR_INVALID, "grouped matmul: leading dimension too small (lda=%lld ldb=%lld ldc=%lld for K=%d N=%d)", (long long)lda,
+                         (long long)ldb, (long long)ldc, K, N);
+    if (groups > 1 && b_outer > 0 && strideB < (b_outer - 1) * ldb + b_inner)
+        return set_error(BTM_ERR_INVALID, "grouped matmul: strideB is smaller than one matrix");
+    if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)C) & 1) return set_error(BTM_ERR_INVALID, "grouped matmul: pointer not aligned to the element size");
+    DeviceState *ds = device_state(device);
+    if (!ds) return last_code();
+    if (groups == 0 || rows == 0 || N == 0) return BTM_OK;
+    GroupedCall c;
+    memset(&c, 0, sizeof(c));
+    c.dtype = dtype; c.b_trans = b_transposed != 0; c.groups = groups; c.rows = rows; c.N = N; c.K = K; c.offsets = offsets;
+    c.A = A; c.lda = lda; c.B = B; c.strideB = strideB; c.ldb = ldb; c.C = C; c.ldc = ldc;
+    return launch_gemm_grouped(c, (cudaStream_t)stream, ds->sm_count, ds->status);
+}
+
+int btm_gemm_grouped_wgrad(int device, void *stream, int dtype, int groups, int rows, int M, int N, const int32_t *offsets, const void *A,
+                           int64_t lda, const void *D, int64_t ldd, void *C, int64_t strideC, int64_t ldc)
+{
+    if (dtype != BTM_F16 && dtype != BTM_BF16)
+        return set_error(BTM_ERR_UNSUPPORTED, "grouped weight gradient: dtype %d is not supported (Float16, BFloat16 only)", dtype);
+    if (M < 0 || N < 0) return set_error(BTM_ERR_INVALID, "grouped weight gradient: negative dimension (M=%d N=%d)", M, N);
+    int rc = check_groups("grouped weight gradient", groups, rows, offsets);
+    if (rc) return rc;
+    if (groups > 0 && M > 0 && N > 0 && (!C || (rows > 0 && (!A || !D)))) return set_error(BTM_ERR_INVALID, "grouped weight gradient: null pointer");
+    if (lda < M || ldd < N || ldc < N)
+        return set_error(BTM_ERR_INVALID, "grouped weight gradient: leading dimension too small (lda=%lld ldd=%lld ldc=%lld for M=%d N=%d)",
+                         (long long)lda, (long long)ldd, (long long)ldc, M, N);
+    if (groups > 1 && M > 0 && strideC < (int64_t)(M - 1) * ldc + N)
+        return set_error(BTM_ERR_INVALID, "grouped weight gradient: strideC is smaller than one matrix");
+    if (((uintptr_t)A | (uintptr_t)D | (uintptr_t)C) & 1) return set_error(BTM_ERR_INVALID, "grouped weight gradient: pointer not aligned to the element size");
+    DeviceState *ds = device_state(device);
+    if (!ds) return last_code();
+    if (groups == 0 || M == 0 || N == 0) return BTM_OK;
+    GroupedCall c;
+    memset(&c, 0, sizeof(c));
+    c.dtype = dtype; c.wgrad = true; c.groups = groups; c.rows = rows; c.M = M; c.N = N; c.offsets = offsets;
+    c.A = A; c.lda = lda; c.B = D; c.ldb = ldd; c.C = C; c.strideC = strideC; c.ldc = ldc;
+    return launch_gemm_grouped(c, (cudaStream_t)stream, ds->sm_count, ds->status);
+}
+
+size_t btm_mxfp4_scale_bytes(int groups, int rows, int K)
+{
+    if (groups <= 0 || rows <= 0 || K <= 0) return 0;
+    return (size_t)grouped_slot_bound(groups, rows) * (size_t)((K + 127LL) / 128) * 512;
+}
+
+static int check_mxfp4(const char *what, int groups, int rows, int K, const void *packed, const void *scales)
+{
+    if (groups < 0 || rows < 0 || K < 0) return set_error(BTM_ERR_INVALID, "%s: negative dimension (groups=%d rows=%d K=%d)", what, groups, rows, K);
+    if (K % 32) return set_error(BTM_ERR_INVALID, "%s: K=%d must be a multiple of 32", what, K);
+    if (groups > 0 && rows > 0 && K > 0 && (!packed || !scales)) return set_error(BTM_ERR_INVALID, "%s: null pointer", what);
+    if (((uintptr_t)packed | (uintptr_t)scales) & 15) return set_error(BTM_ERR_INVALID, "%s: packed values and scales must be 16-byte aligned", what);
+    return BTM_OK;
+}
+
+static int check_mxfp4_convert(const char *what, int dtype, int groups, int rows, int K, const int32_t *offsets, const void *packed,
+                               const void *scales, const void *plain, int64_t ld)
+{
+    if (dtype != BTM_F16 && dtype != BTM_BF16 && dtype != BTM_F32)
+        return set_error(BTM_ERR_UNSUPPORTED, "%s: dtype %d is not supported (Float16, BFloat16, Float32 only)", what, dtype);
+    int rc = check_mxfp4(what, groups, rows, K, packed, scales);
+    if (rc) return rc;
+    if (offsets) {
+        rc = check_groups(what, groups, rows, offsets);
+        if (rc) return rc;
+    } else if (groups > 0 && rows % groups) {
+        return set_error(BTM_ERR_INVALID, "%s: %d rows do not divide into %d equal groups", what, rows, groups);
+    }
+    if (groups > 0 && rows > 0 && K > 0 && !plain) return set_error(BTM_ERR_INVALID, "%s: null pointer", what);
+    if (ld < K) return set_error(BTM_ERR_INVALID, "%s: leading dimension %lld is smaller than K=%d", what, (long long)ld, K);
+    if ((uintptr_t)plain % es_of(dtype)) return set_error(BTM_ERR_INVALID, "%s: pointer not aligned to the element size", what);
+    return BTM_OK;
+}
+
+int btm_mxfp4_quantize(int device, void *stream, int src_dtype, int groups, int rows, int K, const int32_t *offsets, const void *x,
+                       int64_t ldx, void *packed, void *scales)
+{
+    int rc = check_mxfp4_convert("mxfp4 quantise", src_dtype, groups, rows, K, offsets, packed, scales, x, ldx);
+    if (rc) return rc;
+    DeviceState *ds = device_state(device);
+    if (!ds) return last_code();
+    if (groups == 0 || rows == 0 || K == 0) return BTM_OK;
+    return launch_mxfp4_quantize((cudaStream_t)stream, src_dtype, groups, rows, K, offsets, x, ldx, packed, scales, ds->status);
+}
+
+int btm_mxfp4_dequant(int device, void *stream, int dst_dtype, int groups, int rows, int K, const int32_t *offsets, const void *packed,
+                      const void *scales, void *out, int64_t ldo)
+{
+    int rc = check_mxfp4_convert("mxfp4 dequantise", dst_dtype, groups, rows, K, offsets, packed, scales, out, ldo);
+    if (rc) return rc;
+    DeviceState *ds = device_state(device);
+    if (!ds) return last_code();
+    if (groups == 0 || rows == 0 || K == 0) return BTM_OK;
+    return launch_mxfp4_dequant((cudaStream_t)stream, dst_dtype, groups, rows, K, offsets, packed, scales, out, ldo, ds->status);
+}
+
+static int mxfp4_matmul_entry(int device, void *stream, int out_dtype, int groups, int rows, int N, int K, const int32_t *offsets,
+                              const void *act, const void *act_scales, const void *w, const void *w_scales, void *out, int64_t ldo)
+{
+    if (out_dtype != BTM_F16 && out_dtype != BTM_BF16)
+        return set_error(BTM_ERR_UNSUPPORTED, "mxfp4 matmul: output dtype %d is not supported (Float16, BFloat16 only)", out_dtype);
+    if (N < 0) return set_error(BTM_ERR_INVALID, "mxfp4 matmul: negative dimension (N=%d)", N);
+    int rc = check_mxfp4("mxfp4 matmul", groups, rows, K, act, act_scales);
+    if (!rc) rc = check_mxfp4("mxfp4 matmul", groups, N, K, w, w_scales);
+    if (rc) return rc;
+    if (rows > 0 && N > 0 && groups > 0 && !out) return set_error(BTM_ERR_INVALID, "mxfp4 matmul: null output pointer");
+    if (ldo < N) return set_error(BTM_ERR_INVALID, "mxfp4 matmul: leading dimension %lld is smaller than N=%d", (long long)ldo, N);
+    if ((uintptr_t)out & 1) return set_error(BTM_ERR_INVALID, "mxfp4 matmul: pointer not aligned to the element size");
+    DeviceState *ds = device_state(device);
+    if (!ds) return last_code();
+    if (groups == 0 || rows == 0 || N == 0) return BTM_OK;
+    Mxfp4Call c;
+    memset(&c, 0, sizeof(c));
+    c.dtype = out_dtype; c.groups = groups; c.rows = rows; c.N = N; c.K = K; c.offsets = offsets;
+    c.act = act; c.act_scales = act_scales; c.w = w; c.w_scales = w_scales; c.out = out; c.ldo = ldo;
+    return launch_mxfp4_matmul(c, (cudaStream_t)stream, ds->sm_count, ds->status);
+}
+
+int btm_mxfp4_matmul(int device, void *stream, int out_dtype, int M, int N, int K, const void *act, const void *act_scales, const void *w,
+                     const void *w_scales, void *out, int64_t ldo)
+{
+    return mxfp4_matmul_entry(device, stream, out_dtype, 1, M, N, K, nullptr, act, act_scales, w, w_scales, out, ldo);
+}
+
+int btm_mxfp4_matmul_grouped(int device, void *stream, int out_dtype, int groups, int rows, int N, int K, const int32_t *offsets,
+                             const void *act, const void *act_scales, const void *w, const void *w_scales, void *out, int64_t ldo)
+{
+    int rc = check_groups("grouped mxfp4 matmul", groups, rows, offsets);
+    if (rc) return rc;
+    return mxfp4_matmul_entry(device, stream, out_dtype, groups, rows, N, K, offsets, act, act_scales, w, w_scales, out, ldo);
 }
 
 int btm_replicate_rows(int device, void *stream, void *const *bufs, int rank, int nranks, size_t offset_bytes, size_t bytes)

@@ -101,6 +101,35 @@ int launch_int4_gemm_tc(cudaStream_t st, int M, int N, int K, int group, const v
                         int *status, int sm_count);
 int launch_gemm_tc2(int dtype, cudaStream_t st, int sm_count, const CUtensorMap &tmA, const CUtensorMap &tmB, const StoreMaps &cm,
                     const GemmParams &p);
+// One product grouped by expert, or its weight gradient (gemm_grouped.cu).
+struct GroupedCall {
+    int dtype;           // BTM_F16 or BTM_BF16
+    bool wgrad, b_trans; // b_trans: B[g] is stored [N, K] (product only)
+    int groups, rows;
+    int M, N, K;         // product: M unused; weight gradient: C[g] is [M, N], K unused
+    const int *offsets;  // device, groups + 1
+    const void *A, *B;   // weight gradient: B is the output gradient [rows, N]
+    long long lda, ldb, strideB;
+    void *C;
+    long long ldc, strideC;
+};
+int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int *status);
+long long grouped_slot_bound(int groups, int rows);
+// Microscaled 4-bit operands (mxfp4.cu). offsets == NULL: every group has rows / groups rows.
+int launch_mxfp4_quantize(cudaStream_t st, int src_dtype, int groups, int rows, int K, const int *offsets, const void *x, long long ldx,
+                          void *packed, void *scales, int *status);
+int launch_mxfp4_dequant(cudaStream_t st, int dst_dtype, int groups, int rows, int K, const int *offsets, const void *packed,
+                         const void *scales, void *out, long long ldo, int *status);
+// out[r, :] = act[r, :] . w[g]^T for the rows r of group g (offsets == NULL: one group).
+struct Mxfp4Call {
+    int dtype; // of the output: BTM_F16 or BTM_BF16
+    int groups, rows, N, K;
+    const int *offsets;
+    const void *act, *act_scales, *w, *w_scales;
+    void *out;
+    long long ldo;
+};
+int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *status);
 // Fills `cm` for the destinations in `p` (no-op when p.c_vec_ok == 0: the general store path needs no maps).
 int encode_store_maps(StoreMaps *cm, int dtype, const GemmParams &p);
 

@@ -21,6 +21,7 @@ enum WaitCode : int {
     WAIT_EPI_STAGE = 105,
     WAIT_PEER_CTA = 106,
     BOUNDS_STORE = 201, // not a wait: a debug bounds check stopped a store
+    ROWS_OFFSETS = 202, // not a wait: a table of row offsets decreased or left the rows it describes
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }

@@ -112,7 +112,8 @@ int btm_debug_set(const char *key, long long value);
 int btm_init(int device);
 
 /* Reads and clears the device-side status word that kernels set when one of their
- * bounded waits ran out. Synchronises `stream`. Returns BTM_OK or BTM_ERR_TIMEOUT. */
+ * bounded waits ran out, or when a table of row offsets had to be repaired (btm_gemm_grouped). Synchronises
+ * `stream`. Returns BTM_OK, BTM_ERR_TIMEOUT or BTM_ERR_INVALID. */
 int btm_check_device_status(int device, void *stream);
 
 /* Dense matmul C[M,N] = A[M,K] . B[K,N], the op that Ops/Algebra/MatMul/MatMul.h:1-8
@@ -233,6 +234,72 @@ int btm_convert(int device, void *stream, int src_dtype, int dst_dtype, int64_t 
 
 /* Unpack only: int8 out[n,k] = W[n,k] in [-8,7]. */
 int btm_int4_unpack(int device, void *stream, int N, int K, const void *w_packed, void *out_i8);
+
+/* Products grouped by expert, with ragged sizes: the rows of A (and of C) are sorted by group and
+ * offsets[g] .. offsets[g + 1] are the rows of group g, as the counts of a mixture-of-experts router give them:
+ *   C[r, :] = A[r, :] . B[g]   for every row r of group g,   B[g] = B + g * strideB, row-major [K, N].
+ * `b_transposed` != 0: B[g] is stored [N, K] (row-major, ldb >= K) and C[r, :] = A[r, :] . B[g]^T; with the output
+ * gradient in the place of A this is the gradient of the activations. The reference has no such op (not even a stub);
+ * it extends Ops/Algebra/MatMul as btm_bmm does, to batches of unequal height.
+ *   offsets  device memory, groups + 1 values, not decreasing, within [0, rows]; read by the kernel in stream order, so
+ *            it may be the output of work queued before. rows = rows of A and C. Rows in front of offsets[0] and behind
+ *            offsets[groups] belong to no group: they are not read and C keeps what it held there. A group may be
+ *            empty. Entries that break these rules never lead outside the operands: they are clamped to [0, rows], an
+ *            entry smaller than an earlier one counts as that earlier one, and the next btm_check_device_status
+ *            returns BTM_ERR_INVALID.
+ * dtype BTM_F16 or BTM_BF16, fp32 accumulation, one rounding. lda >= K, ldc >= N. Alignment as btm_gemm: operands that
+ * the tensor-core path cannot address take a general kernel. One launch, nothing allocated, no host synchronisation;
+ * it can be captured into a graph and replayed with another table. */
+int btm_gemm_grouped(int device, void *stream, int dtype, int groups, int rows, int N, int K, const int32_t *offsets, const void *A,
+                     int64_t lda, const void *B, int64_t strideB, int64_t ldb, int b_transposed, void *C, int64_t ldc);
+
+/* The weight gradient of btm_gemm_grouped: C[g] = A[rows of g]^T . D[rows of g], C[g] = C + g * strideC, row-major
+ * [M, N], where A is [rows, M] (the activations, lda >= M) and D is [rows, N] (the output gradient, ldd >= N). A group
+ * without rows gets an all-zero C[g]; values of rows that belong to no group or to another one never enter, whatever
+ * they are. offsets, dtype and alignment as above. */
+int btm_gemm_grouped_wgrad(int device, void *stream, int dtype, int groups, int rows, int M, int N, const int32_t *offsets, const void *A,
+                           int64_t lda, const void *D, int64_t ldd, void *C, int64_t strideC, int64_t ldc);
+
+/* Microscaled 4-bit floating point (OCP MX, MXFP4). Along k, 32 consecutive values share one power-of-two scale.
+ *   elements  E2M1, [rows, K/2] bytes, even k in bits 0-3: codes 0..7 are 0, .5, 1, 1.5, 2, 3, 4, 6, bit 3 is the sign
+ *   scales    E8M0, one byte s per 32 values, factor 2^(s - 127), 255 = NaN. They are kept in blocks of 128 rows x 4
+ *             scales (128 k), 512 bytes each: block (R, C) at index R * ceil(K/128) + C, and inside it the scale c of
+ *             row r at byte (r % 32) * 16 + (r / 32) * 4 + c; bytes outside the matrix are 0. This is the order in
+ *             which the tensor core takes them, so a product moves them as they lie. The rows of a grouped operand are
+ *             cut per group: group g takes ceil(rows of g / 128) row blocks behind those of the groups before it.
+ * K % 32 == 0; `packed` and `scales` 16-byte aligned. The reference has no quantised type (Tensor/Dtypes.h:57-70);
+ * these are the convert_gpu() cases (Tensor/TensorOps.cu:315-365) and the product for one, as the int4 calls are for
+ * theirs.
+ *
+ * btm_mxfp4_scale_bytes: bytes that hold the scales of `rows` rows in `groups` groups, however the rows are divided. */
+size_t btm_mxfp4_scale_bytes(int groups, int rows, int K);
+
+/* Quantise x [rows, K] (BTM_F32, BTM_F16 or BTM_BF16, ldx >= K): per block X = floor(log2(max|x|)) - 2 clamped to
+ * [-127, 127], codes x / 2^X rounded to nearest (ties to the even code) and saturated at 6. A block with an infinity or
+ * a NaN gets scale 255 and zero codes. offsets == NULL: `groups` groups of rows / groups rows each (the weights of all
+ * experts in one call; rows % groups == 0). Otherwise ragged groups as in btm_gemm_grouped; rows outside the groups are
+ * not read and their codes are left as they were. */
+int btm_mxfp4_quantize(int device, void *stream, int src_dtype, int groups, int rows, int K, const int32_t *offsets, const void *x,
+                       int64_t ldx, void *packed, void *scales);
+
+/* The inverse: out [rows, K] = code * 2^X, rounded once to BTM_F32, BTM_F16 or BTM_BF16 (ldo >= K); NaN where the scale
+ * is. groups and offsets as above; rows outside the groups are left as they were. */
+int btm_mxfp4_dequant(int device, void *stream, int dst_dtype, int groups, int rows, int K, const int32_t *offsets, const void *packed,
+                      const void *scales, void *out, int64_t ldo);
+
+/* Product of two microscaled operands: out[M, N] = act[M, K] . w[N, K]^T, both as btm_mxfp4_quantize writes them
+ * (groups = 1), fp32 accumulation of exact products on the tensor cores, one rounding to out_dtype (BTM_F16 or
+ * BTM_BF16). ldo >= N. Any M >= 0 (a single token included) and N.
+ * Ordering: launched with programmatic stream serialisation like the other products; all operands are read after the
+ * predecessor on the stream has completed. */
+int btm_mxfp4_matmul(int device, void *stream, int out_dtype, int M, int N, int K, const void *act, const void *act_scales, const void *w,
+                     const void *w_scales, void *out, int64_t ldo);
+
+/* The same for experts: out[r, :] = act[r, :] . w[g]^T for the rows r of group g; w is [groups, N, K/2] and w_scales
+ * [groups, ceil(N/128) * ceil(K/128) * 512], as one btm_mxfp4_quantize call with offsets == NULL and groups * N rows writes
+ * them; act and act_scales come from one with these offsets. Rows outside the groups as in btm_gemm_grouped. */
+int btm_mxfp4_matmul_grouped(int device, void *stream, int out_dtype, int groups, int rows, int N, int K, const int32_t *offsets,
+                             const void *act, const void *act_scales, const void *w, const void *w_scales, void *out, int64_t ldo);
 
 /* N-sharded matmul with the all-gather fused into the epilogue: this rank holds all of A
  * and the column block B[:, rank*Nloc:(rank+1)*Nloc]; it computes C[:, that block] and
