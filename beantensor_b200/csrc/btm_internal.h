@@ -113,6 +113,7 @@ struct GroupedCall {
     void *C;
     long long ldc, strideC;
 };
+int configure_gemm_grouped_kernels();
 int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int *status);
 long long grouped_slot_bound(int groups, int rows);
 // Microscaled 4-bit operands (mxfp4.cu). offsets == NULL: every group has rows / groups rows.

@@ -3,6 +3,21 @@
 //   product:          C[r, :] = A[r, :] . B[g]                   r in group g
 //   weight gradient:  C[g]    = A[rows of g]^T . D[rows of g]    (all zero for a group without rows)
 //
+// Tensor-core kernel: one persistent CTA per SM with the warp roles of gemm_tc.cu (TMA producer, tcgen05.mma issuer with
+// two accumulators in tensor memory, four epilogue warps). What differs is where a tile's rows come from: every role
+// walks the table by itself, a warp at a time, and no tile list exists in memory.
+//   product    rows are cut per group into slots of 128; a tile is (slot, column range). A tile reads up to 128 rows of
+//              A from the group's first row on, whatever alignment that has (a row coordinate is free), so rows of the
+//              next group can be in it: each only spoils its own output row, which is not stored. Bands of 32 rows that
+//              lie inside the group leave by TMA store, the band that the group's end cuts by 16-byte stores of
+//              its own rows.
+//   gradient   a tile is (group, row range of C, column range), its k-blocks are 64 rows of the group. Both operands are
+//              MN-major as they lie. The last k-block is cut: rows behind the group's end are overwritten with zero in
+//              both operands in shared memory (zero times a foreign infinity would be NaN), and only the 16-row steps that
+//              hold rows of the group are multiplied.
+// Few tiles or a ragged last wave: the tile width (256, 128 or 64 columns, and half of it for what would be a partly
+// filled last wave) is chosen on the device from the number of slots, by the same rule in every CTA.
+//
 // General kernel (operands that TMA cannot address, K == 0): 64 x 64 output tiles on CUDA cores as in gemm_simt.cu, fp32
 // accumulation, one rounding. A block finds its group by walking the table.
 #include <cstring>
@@ -12,9 +27,367 @@
 
 #include "btm_internal.h"
 #include "btm_ptx.cuh"
+#include "gemm_epilogue.cuh"
 #include "grouped_rows.cuh"
 
 namespace btm {
+
+enum GroupedMode { GROUPED_KN = 0 /* B[g] is [K, N] */, GROUPED_NK = 1 /* B[g] is [N, K] */, GROUPED_WGRAD = 2 };
+
+namespace gg {
+constexpr int BM = 128;                 // rows of an output tile = accumulator lanes
+constexpr int BN = 256;                 // widest tile
+constexpr int BK = 64;                  // k per stage: 128 bytes
+constexpr int CHUNK_BYTES = 64 * 128;   // every TMA box of an operand is 64 rows x 128 bytes, except A of the product
+constexpr int A_BYTES = BM * 128;
+constexpr int STAGE_BYTES = A_BYTES + BN * 128;
+constexpr int STAGES = 4;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_SMEM_BYTES + 1024;
+constexpr int TMEM_COLS = 512;
+constexpr int THREADS = 192;
+constexpr int A_BAND = 32;              // rows of a short A box: a tile with few rows does not fetch its neighbours'
+} // namespace gg
+
+struct GroupedTables {
+    const int *offsets;
+    int groups, rows;
+};
+
+// How the tiles of a launch are cut, from the number of slots: the same in every warp of the grid.
+struct GroupedPlan {
+    int bn, tiles_n;  // tile width and tiles per slot
+    int full, total;  // tiles of that width, then (total - full) of half of it
+};
+
+// Cost of a tile in units of B columns: its columns plus kTileOverhead for what does not shrink with the width (the A
+// rows, the hand-offs). Waves are counted whole, a last one that fits twice over is run as half-width tiles.
+__device__ __forceinline__ GroupedPlan plan_tiles(int slots, int N, int ctas)
+{
+    constexpr int kTileOverhead = 64;
+    GroupedPlan best;
+    long long best_cost = 0x7FFFFFFFFFFFFFFFLL;
+#pragma unroll
+    for (int bn = gg::BN; bn >= 64; bn >>= 1) {
+        const int tiles_n = (N + bn - 1) / bn;
+        const int tiles = slots * tiles_n;
+        const int waves = tiles / ctas, rem = tiles - waves * ctas;
+        const bool halves = bn >= 128 && rem > 0 && 2 * rem <= ctas;
+        const long long cost = (long long)waves * (bn + kTileOverhead) + (rem == 0 ? 0 : (halves ? bn / 2 : bn) + kTileOverhead);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best.bn = bn;
+            best.tiles_n = tiles_n;
+            best.full = halves ? tiles - rem : tiles;
+            best.total = halves ? tiles + rem : tiles;
+        }
+    }
+    return best;
+}
+
+struct GroupedTile {
+    int g, lo, hi; // group and its rows
+    int m0;        // first output row (row of A for the product, row of C[g] for the gradient)
+    int n0, bn;    // columns
+};
+
+template <int MODE>
+__device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const GroupedPlan &pl, GroupWalk &walk, int t)
+{
+    GroupedTile o;
+    int tile = t, half = -1;
+    if (t >= pl.full) {
+        const int s = t - pl.full;
+        tile = pl.full + (s >> 1);
+        half = s & 1;
+    }
+    const int slot = tile / pl.tiles_n;
+    int first, count; // the group's slots
+    if (MODE == GROUPED_WGRAD) {
+        o.g = slot / p.tiles_m;
+        first = o.g * p.tiles_m;
+        count = p.tiles_m;
+        walk.find_group(o.g, o.lo, o.hi);
+    } else {
+        walk.find_slot(slot, o.g, o.lo, o.hi, first);
+        count = (o.hi - o.lo + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS;
+    }
+    // Within a group: bands of group_m row tiles, row tiles innermost, so that neighbouring CTAs share columns of B.
+    const int r0 = tile - first * pl.tiles_n;
+    const int per_band = p.group_m * pl.tiles_n;
+    const int band = r0 / per_band;
+    const int first_m = band * p.group_m;
+    const int height = min(count - first_m, p.group_m);
+    const int r = r0 - band * per_band;
+    o.m0 = (MODE == GROUPED_WGRAD ? 0 : o.lo) + (first_m + r % height) * gg::BM;
+    o.bn = half < 0 ? pl.bn : pl.bn / 2;
+    o.n0 = (r / height) * pl.bn + (half > 0 ? pl.bn / 2 : 0);
+    return o;
+}
+
+// One 32-row band of a finished tile to C. `rows_end`: rows from here on are not this tile's. zero: the sum is empty.
+template <int DT, int MODE>
+__device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensorMap &tmC, uint32_t tmem_band, const GroupedTile &t, int row0,
+                                             int rows_end, bool zero, uint32_t epi_smem, uint32_t &tile_count, int lane)
+{
+    if (row0 >= rows_end) return;
+    const int z = MODE == GROUPED_WGRAD ? t.g : 0;
+    const long long base = (long long)z * p.strideC;
+    if (!p.c_vec_ok) {
+        const int row = row0 + lane;
+#pragma unroll 1
+        for (int c = 0; c < t.bn / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32(tmem_band + (uint32_t)(c * 32), v);
+            tmem_ld_wait();
+            if (zero) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0u;
+            }
+            const int col = t.n0 + c * 32, valid = min(32, p.N - col);
+            if (row < rows_end && valid > 0) store_row_direct<DT>(p, v, base + (long long)row * p.ldc + col, valid);
+        }
+        return;
+    }
+    const uint32_t swz = (uint32_t)(lane & 7);
+    const bool whole = MODE == GROUPED_WGRAD || row0 + 32 <= rows_end; // C[g] is clipped by its tensor map
+#pragma unroll 1
+    for (int c = 0; c < t.bn / 64; ++c) {
+        const int col = t.n0 + c * 64;
+        if (col >= p.N) break;
+        const uint32_t buf = epi_smem + (tile_count & 1u) * EPI_TILE_BYTES;
+        ++tile_count;
+        if (lane == 0) bulk_wait_read<1>();
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t v[32], q[16];
+            tmem_ld_32x32(tmem_band + (uint32_t)(c * 64 + h * 32), v);
+            tmem_ld_wait();
+            pack16<DT>(v, q);
+            if (zero) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) q[j] = 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                st_shared_v4(buf + (uint32_t)lane * 128u + (((uint32_t)(h * 4 + j) ^ swz) << 4), q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
+        }
+        if (whole) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_3d(&tmC, buf, col, row0, z);
+                bulk_commit();
+            }
+        } else {
+            __syncwarp();
+            uint16_t *dst = reinterpret_cast<uint16_t *>(p.C[0]);
+            const int j = lane & 7, ccol = col + j * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3), row = row0 + r;
+                if (row < rows_end && ccol < p.N) {
+                    uint4 v;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                 : "r"(buf + (uint32_t)r * 128u + (((uint32_t)(j ^ (r & 7))) << 4)));
+                    const long long off = base + (long long)row * p.ldc + ccol;
+                    if (store_in_bounds(p, off, min(8, p.N - ccol))) {
+                        if (ccol + 8 <= p.N) {
+                            *reinterpret_cast<uint4 *>(dst + off) = v;
+                        } else {
+                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (ccol + e < p.N) dst[off + e] = (uint16_t)((e & 1) ? (w[e >> 1] >> 16) : (w[e >> 1] & 0xFFFFu));
+                        }
+                    }
+                }
+            }
+            if (lane == 0) bulk_commit(); // an empty group keeps the buffer accounting uniform
+        }
+    }
+}
+
+// tmA: 128-row boxes (product) or 64-row boxes (gradient); tmA_band: boxes of A_BAND rows (product only).
+template <int DT, int MODE>
+__global__ void __launch_bounds__(gg::THREADS, 1)
+gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA_band, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmC, const __grid_constant__ GemmParams p, const GroupedTables tab)
+{
+    using namespace gg;
+    constexpr bool kWgrad = MODE == GROUPED_WGRAD;
+    constexpr bool kBMnMajor = MODE != GROUPED_NK;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bar_full[STAGES], bar_empty[STAGES], bar_tmem_full[2], bar_tmem_empty[2];
+    __shared__ uint32_t tmem_base_holder;
+    __shared__ int abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(smem_u32(&bar_full[s]), 1);
+            mbar_init(smem_u32(&bar_empty[s]), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(smem_u32(&bar_tmem_full[a]), 1);
+            mbar_init(smem_u32(&bar_tmem_empty[a]), 4);
+        }
+        fence_mbar_init();
+        prefetch_tmap(&tmA);
+        prefetch_tmap(&tmB);
+        if (!kWgrad) prefetch_tmap(&tmA_band);
+    }
+    if (warp == 1) {
+        tmem_alloc<1>(smem_u32(&tmem_base_holder), TMEM_COLS);
+        tmem_relinquish<1>();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_holder;
+    // Everything behind this line reads what earlier work on the stream may have written, the table first of all; only
+    // then may a successor be let in, which so can rely on this grid's predecessors.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    GroupWalk walk;
+    walk.init(tab.offsets, tab.groups, tab.rows);
+    const int group_slots = walk.count_slots();
+    if (blockIdx.x == 0 && warp == 0) walk.report(p.status);
+    const GroupedPlan plan = plan_tiles(kWgrad ? tab.groups * p.tiles_m : group_slots, p.N, gridDim.x);
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = !p.debug_skip_loads;
+        for (int tile = blockIdx.x; ok && tile < plan.total; tile += gridDim.x) {
+            const GroupedTile t = grouped_tile<MODE>(p, plan, walk, tile);
+            const int num_kb = kWgrad ? (t.hi - t.lo + BK - 1) / BK : p.num_kb;
+            const int chunks = t.bn / 64;
+            const int bands = min(4, (t.hi - t.m0 + A_BAND - 1) / A_BAND); // of A rows that the tile owns (product)
+            const uint32_t bytes = (uint32_t)((kWgrad || bands == 4 ? A_BYTES : bands * A_BAND * 128) + chunks * CHUNK_BYTES);
+            for (int kb = 0; kb < num_kb; ++kb) {
+                ok = mbar_wait_warp(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
+                if (!ok) break;
+                if (lane == 0) {
+                    const uint32_t full = smem_u32(&bar_full[stage]);
+                    const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
+                    const int k0 = kWgrad ? t.lo + kb * BK : kb * BK;
+                    mbar_expect_tx(full, bytes);
+                    if constexpr (kWgrad) {
+                        tma_load_3d(a0, &tmA, t.m0, k0, 0, full);
+                        tma_load_3d(a0 + CHUNK_BYTES, &tmA, t.m0 + 64, k0, 0, full);
+                    } else if (bands == 4) {
+                        tma_load_3d(a0, &tmA, k0, t.m0, 0, full);
+                    } else {
+                        for (int b = 0; b < bands; ++b) tma_load_3d(a0 + b * A_BAND * 128, &tmA_band, k0, t.m0 + b * A_BAND, 0, full);
+                    }
+                    const int zb = kWgrad ? 0 : t.g;
+                    for (int c = 0; c < chunks; ++c) {
+                        if (kBMnMajor) tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, t.n0 + c * 64, k0, zb, full);
+                        else tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, k0, t.n0 + c * 64, zb, full);
+                    }
+                }
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        constexpr uint32_t kFmt = DT == BTM_BF16 ? 1u : 0u;
+        constexpr uint32_t a_step = (kWgrad ? 16 * 128 : 32) >> 4, b_step = (kBMnMajor ? 16 * 128 : 32) >> 4; // 16 k, in 16-byte units
+        int stage = 0, it = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < plan.total; tile += gridDim.x, ++it) {
+            const GroupedTile t = grouped_tile<MODE>(p, plan, walk, tile);
+            const int num_kb = kWgrad ? (t.hi - t.lo + BK - 1) / BK : p.num_kb;
+            const uint32_t idesc = make_idesc(kFmt, kWgrad, kBMnMajor, BM, (uint32_t)t.bn);
+            const int acc = it & 1;
+            ok = mbar_wait_warp(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+            for (int kb = 0; kb < num_kb; ++kb) {
+                ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
+                if (!ok) break;
+                const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
+                int steps = BK / 16;
+                if (kWgrad) {
+                    const int left = t.hi - t.lo - kb * BK; // rows of the group in this k-block
+                    if (left < BK) {
+                        steps = (left + 15) / 16;
+                        // Rows left .. 16 * steps - 1 of every 64-wide chunk: 128 contiguous bytes per row.
+                        const int dirty = steps * 16 - left;
+                        for (int i = lane; i < dirty * 8; i += 32) {
+                            const uint32_t off = (uint32_t)(left + (i >> 3)) * 128u + (uint32_t)(i & 7) * 16u;
+                            for (int c = 0; c < BM / 64; ++c) st_shared_v4(a0 + c * CHUNK_BYTES + off, 0u, 0u, 0u, 0u);
+                            for (int c = 0; c < t.bn / 64; ++c) st_shared_v4(b0 + c * CHUNK_BYTES + off, 0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
+                tc_fence_after();
+                const uint64_t ad = kWgrad ? make_smem_desc_sw128(a0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(a0, 16, 1024);
+                const uint64_t bd = kBMnMajor ? make_smem_desc_sw128(b0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(b0, 16, 1024);
+                if (elect_one()) {
+#pragma unroll
+                    for (int ks = 0; ks < BK / 16; ++ks)
+                        if (!kWgrad || ks < steps)
+                            umma<1, false>(d_tmem, ad + (uint64_t)(ks * a_step), bd + (uint64_t)(ks * b_step), idesc, (uint32_t)((kb | ks) != 0));
+                    umma_commit(smem_u32(&bar_empty[stage]));
+                }
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (ok && elect_one()) umma_commit(smem_u32(&bar_tmem_full[acc]));
+            __syncwarp();
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue (warps 2..5)
+        const int quad = warp & 3;
+        const uint32_t epi_smem = smem_base + STAGES * STAGE_BYTES + (uint32_t)quad * EPI_WARP_BYTES;
+        uint32_t epi_tiles = 0;
+        int it = 0;
+        for (int tile = blockIdx.x; tile < plan.total; tile += gridDim.x, ++it) {
+            const GroupedTile t = grouped_tile<MODE>(p, plan, walk, tile);
+            const int acc = it & 1;
+            if (!mbar_wait_warp(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
+            tc_fence_after();
+            grouped_band<DT, MODE>(p, tmC, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t, t.m0 + quad * 32,
+                                   kWgrad ? p.M : t.hi, kWgrad && t.lo == t.hi, epi_smem, epi_tiles, lane);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));
+        }
+        epilogue_drain(lane);
+    }
+
+    // ---------------------------------------------------------------- teardown
+    tc_fence_before();
+    __syncthreads();
+    if (abort_flag) {
+        // A wait ran out somewhere: copies in flight land within microseconds, shared memory is held that long.
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+        __syncthreads();
+    }
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc<1>(tmem_base, TMEM_COLS);
+    }
+}
 
 template <int DT>
 struct Half16;
@@ -162,10 +535,101 @@ static int launch_grouped_simt(const GroupedCall &c, cudaStream_t st, int *statu
     return check_cuda(cudaGetLastError(), "grouped matmul (general kernel) launch");
 }
 
+template <int DT, int MODE>
+static int launch_tc(const GroupedCall &c, cudaStream_t st, int grid, const CUtensorMap &tmA, const CUtensorMap &tmA_band, const CUtensorMap &tmB,
+                     const CUtensorMap &tmC, const GemmParams &p)
+{
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)grid, 1, 1);
+    cfg.blockDim = dim3(gg::THREADS, 1, 1);
+    cfg.dynamicSmemBytes = gg::SMEM_BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    GroupedTables tab = {c.offsets, c.groups, c.rows};
+    return check_cuda(cudaLaunchKernelEx(&cfg, gemm_grouped_kernel<DT, MODE>, tmA, tmA_band, tmB, tmC, p, tab), "grouped matmul launch");
+}
+
+template <int DT>
+static cudaError_t raise_grouped_smem()
+{
+    cudaError_t e = cudaFuncSetAttribute(gemm_grouped_kernel<DT, GROUPED_KN>, cudaFuncAttributeMaxDynamicSharedMemorySize, gg::SMEM_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(gemm_grouped_kernel<DT, GROUPED_NK>, cudaFuncAttributeMaxDynamicSharedMemorySize, gg::SMEM_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(gemm_grouped_kernel<DT, GROUPED_WGRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, gg::SMEM_BYTES);
+    return e;
+}
+
+int configure_gemm_grouped_kernels()
+{
+    cudaError_t e = raise_grouped_smem<BTM_F16>();
+    if (e == cudaSuccess) e = raise_grouped_smem<BTM_BF16>();
+    return check_cuda(e, "cudaFuncSetAttribute(gemm_grouped)");
+}
+
+static bool mult16(const void *p, long long ld) { return ((uintptr_t)p & 15) == 0 && (ld * 2) % 16 == 0; }
+
 int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int *status)
 {
-    (void)sm_count;
-    return launch_grouped_simt(c, st, status);
+    using namespace gg;
+    // Tensor maps take bases and pitches that are multiples of 16 bytes; anything else, an empty reduction and a matrix
+    // without rows take the general kernel.
+    const bool tc = mult16(c.A, c.lda) && mult16(c.B, c.ldb) && (c.wgrad || c.groups == 1 || (c.strideB * 2) % 16 == 0) && c.rows > 0 &&
+                    (c.wgrad || c.K > 0);
+    if (!tc) return launch_grouped_simt(c, st, status);
+    const long long bound = c.wgrad ? (long long)c.groups * ((c.M + BM - 1) / BM) : grouped_slot_bound(c.groups, c.rows);
+    const long long most = bound * ((c.N + 63) / 64); // tiles at the smallest width
+    if (most > 0x3FFFFFFFLL) return set_error(BTM_ERR_UNSUPPORTED, "grouped matmul: too many output tiles (%lld)", most);
+
+    CUtensorMap tmA, tmA_band, tmB, tmC;
+    memset(&tmA_band, 0, sizeof(tmA_band));
+    memset(&tmC, 0, sizeof(tmC));
+    const uint64_t rows = (uint64_t)c.rows, pa = (uint64_t)c.lda * 2, pb = (uint64_t)c.ldb * 2;
+    int rc;
+    if (c.wgrad) {
+        rc = encode_tmap_3d(&tmA, c.dtype, c.A, (uint64_t)c.M, rows, 1, pa, pa, 64, 64);
+        if (!rc) rc = encode_tmap_3d(&tmB, c.dtype, c.B, (uint64_t)c.N, rows, 1, pb, pb, 64, 64);
+    } else {
+        rc = encode_tmap_3d(&tmA, c.dtype, c.A, (uint64_t)c.K, rows, 1, pa, pa, 64, BM);
+        if (!rc) rc = encode_tmap_3d(&tmA_band, c.dtype, c.A, (uint64_t)c.K, rows, 1, pa, pa, 64, A_BAND);
+        const uint64_t inner = (uint64_t)(c.b_trans ? c.K : c.N), outer = (uint64_t)(c.b_trans ? c.N : c.K);
+        if (!rc) rc = encode_tmap_3d(&tmB, c.dtype, c.B, inner, outer, (uint64_t)c.groups, pb, c.groups > 1 ? (uint64_t)c.strideB * 2 : pb, 64, 64);
+    }
+    if (rc) return rc;
+    GemmParams p;
+    memset(&p, 0, sizeof(p));
+    p.M = c.wgrad ? c.M : c.rows;
+    p.N = c.N;
+    p.K = c.K;
+    p.batch = c.wgrad ? c.groups : 1;
+    p.tiles_m = c.wgrad ? (c.M + BM - 1) / BM : 0;
+    p.num_kb = (c.K + BK - 1) / BK;
+    p.group_m = 8; // as in gemm_tc.cu
+    p.ndst = 1;
+    p.C[0] = c.C;
+    p.ldc = c.ldc;
+    p.strideC = c.strideC;
+    p.c_vec_ok = mult16(c.C, c.ldc) && (!c.wgrad || c.groups == 1 || (c.strideC * 2) % 16 == 0) ? 1 : 0;
+    p.status = status;
+    fill_wait_params(&p);
+    if (p.c_vec_ok) {
+        const uint64_t pc = (uint64_t)c.ldc * 2;
+        rc = encode_tmap_3d(&tmC, c.dtype, c.C, (uint64_t)c.N, (uint64_t)p.M, (uint64_t)p.batch, pc, p.batch > 1 ? (uint64_t)c.strideC * 2 : pc, 64, 32);
+        if (rc) return rc;
+    }
+    const int grid = (int)(most < sm_count ? most : sm_count);
+#define BTM_GROUPED_CASE(DT)                                                                                    \
+    do {                                                                                                        \
+        if (c.wgrad) return launch_tc<DT, GROUPED_WGRAD>(c, st, grid, tmA, tmA_band, tmB, tmC, p);              \
+        if (c.b_trans) return launch_tc<DT, GROUPED_NK>(c, st, grid, tmA, tmA_band, tmB, tmC, p);               \
+        return launch_tc<DT, GROUPED_KN>(c, st, grid, tmA, tmA_band, tmB, tmC, p);                              \
+    } while (0)
+    if (c.dtype == BTM_F16) BTM_GROUPED_CASE(BTM_F16);
+    BTM_GROUPED_CASE(BTM_BF16);
+#undef BTM_GROUPED_CASE
 }
 
 } // namespace btm

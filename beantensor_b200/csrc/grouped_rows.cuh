@@ -74,8 +74,9 @@ struct GroupWalk {
     // The group that holds `slot`, which must be below count_slots() and not below the slot of an earlier call.
     __device__ __forceinline__ void find_slot(int slot, int &group, int &row_lo, int &row_hi, int &first_slot)
     {
-        while (slot >= slots_before + __shfl_sync(0xffffffffu, incl, 31)) next();
-        const int l = __ffs(__ballot_sync(0xffffffffu, slots_before + incl > slot)) - 1;
+        // (The walk ends with the table whatever happens to it meanwhile; lane 0 then stands in for a group not found.)
+        while (g0 + 32 < groups && slot >= slots_before + __shfl_sync(0xffffffffu, incl, 31)) next();
+        const int l = max(0, __ffs(__ballot_sync(0xffffffffu, slots_before + incl > slot)) - 1);
         group = g0 + l;
         row_lo = __shfl_sync(0xffffffffu, lo, l);
         row_hi = __shfl_sync(0xffffffffu, hi, l);
