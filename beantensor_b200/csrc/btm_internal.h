@@ -130,6 +130,7 @@ struct Mxfp4Call {
     void *out;
     long long ldo;
 };
+int configure_mxfp4_kernels();
 int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *status);
 // Fills `cm` for the destinations in `p` (no-op when p.c_vec_ok == 0: the general store path needs no maps).
 int encode_store_maps(StoreMaps *cm, int dtype, const GemmParams &p);

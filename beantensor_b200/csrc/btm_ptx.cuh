@@ -183,6 +183,14 @@ __device__ __forceinline__ void tma_load_3d_2sm(uint32_t dst, const CUtensorMap 
         : "memory");
 }
 
+// Untiled bulk copy global -> this CTA's shared memory; addresses and size are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(bar)
+                 : "memory");
+}
+
 // ---------------------------------------------------------------- tcgen05 / tensor memory
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -254,6 +262,35 @@ __device__ __forceinline__ void umma_a_tmem(uint32_t d_tmem, uint32_t a_tmem, ui
         : "memory");
 }
 
+// Microscaled 4-bit product (kind::mxf4, K = 64 per instruction, one E8M0 scale per 32 k): the scales of both operands lie
+// in tensor memory at sfa / sfb, which of a column's two pairs of bytes is meant is in the instruction descriptor.
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate)
+{
+    if constexpr (kCtaGroup == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+// Shared memory -> tensor memory: 32 rows of 16 bytes become 4 columns of 32 lanes, repeated in all four lane quadrants.
+// Ordered before tcgen05.mma issued later by the same thread.
+template <int kCtaGroup>
+__device__ __forceinline__ void tmem_cp_32x128b(uint32_t taddr, uint64_t s_desc)
+{
+    if constexpr (kCtaGroup == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+}
+
 // Make `bar` (in this CTA) observe completion of all tcgen05.mma issued so far by this thread.
 __device__ __forceinline__ void umma_commit(uint32_t bar)
 {
@@ -307,6 +344,20 @@ __host__ __device__ constexpr uint64_t make_smem_desc_sw128(uint32_t smem_addr, 
 {
     return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16) |
            ((uint64_t)((sbo_bytes >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// The same without swizzle for rows of 16 bytes: 8-row groups of 128 contiguous bytes, 128 bytes apart.
+__host__ __device__ constexpr uint64_t make_smem_desc_rows16(uint32_t smem_addr)
+{
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128u >> 4) << 16) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46);
+}
+
+// Instruction descriptor (32 bit) for kind::mxf4: A and B format 1 (E2M1) in [7,10) and [10,12), both K-major; N >> 3 in
+// [17,23); scale format 1 (E8M0) in bit 23; M >> 7 in [27,29); the pair of scale bytes (0 or 2) of A in [29,31) and of
+// B in [4,6).
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(uint32_t M, uint32_t N, uint32_t pair)
+{
+    return (pair << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | (1u << 23) | ((M >> 7) << 27) | (pair << 29);
 }
 
 // Instruction descriptor (32 bit) for kind::f16 / kind::tf32 with fp32 accumulation:

@@ -13,7 +13,7 @@ namespace btm {
 
 constexpr int GROUP_SLOT_ROWS = 128; // a group's rows are cut into slots of this many rows, the last one short
 
-// All members are used by a whole warp at once.
+// All members are used by a whole warp at once. Without a table there is one group that owns every row.
 struct GroupWalk {
     const int *offsets;
     int groups, rows;
@@ -29,7 +29,7 @@ struct GroupWalk {
         floor_row = floor_at;
         slots_before = slots;
         int raw = floor_at;
-        if (first + lane < groups) raw = offsets[first + lane + 1];
+        if (first + lane < groups) raw = offsets ? offsets[first + lane + 1] : rows;
         hi = min(max(raw, floor_at), rows);
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -50,7 +50,7 @@ struct GroupWalk {
 
     __device__ __forceinline__ void first_window()
     {
-        const int raw = offsets[0], at = min(max(raw, 0), rows);
+        const int raw = offsets ? offsets[0] : 0, at = min(max(raw, 0), rows);
         bad |= raw != at ? 1 : 0;
         load(0, at, 0);
     }

@@ -1,0 +1,174 @@
+// Tiles of grouped products: how the slots and columns of all groups are cut into tiles, which rows and columns a tile
+// has, and its way from tensor memory to C. Used by the 16-bit kernels (gemm_grouped.cu) and by the microscaled one
+// (mxfp4_tc.cu).
+#pragma once
+#include "gemm_epilogue.cuh"
+#include "grouped_rows.cuh"
+
+namespace btm {
+
+struct GroupedTables {
+    const int *offsets;
+    int groups, rows;
+};
+
+// How the tiles of a launch are cut, from the number of slots: the same in every warp of the grid.
+struct GroupedPlan {
+    int bn, tiles_n;  // tile width and tiles per slot
+    int full, total;  // tiles of that width, then (total - full) of half of it
+};
+
+// Cost of a tile in units of B columns: its columns plus kTileOverhead for what does not shrink with the width (the A
+// rows, the hand-offs). Waves are counted whole, a last one that fits twice over is run as half-width tiles.
+template <int kWidest>
+__device__ __forceinline__ GroupedPlan plan_tiles(int slots, int N, int ctas)
+{
+    constexpr int kTileOverhead = 64;
+    GroupedPlan best;
+    long long best_cost = 0x7FFFFFFFFFFFFFFFLL;
+#pragma unroll
+    for (int bn = kWidest; bn >= 64; bn = bn > 128 ? 128 : bn / 2) {
+        const int tiles_n = (N + bn - 1) / bn;
+        const int tiles = slots * tiles_n;
+        const int waves = tiles / ctas, rem = tiles - waves * ctas;
+        const bool halves = bn % 128 == 0 && rem > 0 && 2 * rem <= ctas;
+        const long long cost = (long long)waves * (bn + kTileOverhead) + (rem == 0 ? 0 : (halves ? bn / 2 : bn) + kTileOverhead);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best.bn = bn;
+            best.tiles_n = tiles_n;
+            best.full = halves ? tiles - rem : tiles;
+            best.total = halves ? tiles + rem : tiles;
+        }
+    }
+    return best;
+}
+
+struct GroupedTile {
+    int g, lo, hi; // group and its rows
+    int slot;      // its slot, counted over all groups (product)
+    int m0;        // first output row (row of A for the product, row of C[g] for the gradient)
+    int n0, bn;    // columns
+};
+
+template <bool kWgrad>
+__device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const GroupedPlan &pl, GroupWalk &walk, int t)
+{
+    GroupedTile o;
+    int tile = t, half = -1;
+    if (t >= pl.full) {
+        const int s = t - pl.full;
+        tile = pl.full + (s >> 1);
+        half = s & 1;
+    }
+    const int slot = tile / pl.tiles_n;
+    int first, count; // the group's slots
+    if (kWgrad) {
+        o.g = slot / p.tiles_m;
+        first = o.g * p.tiles_m;
+        count = p.tiles_m;
+        walk.find_group(o.g, o.lo, o.hi);
+    } else {
+        walk.find_slot(slot, o.g, o.lo, o.hi, first);
+        count = (o.hi - o.lo + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS;
+    }
+    // Within a group: bands of group_m row tiles, row tiles innermost, so that neighbouring CTAs share columns of B.
+    const int r0 = tile - first * pl.tiles_n;
+    const int per_band = p.group_m * pl.tiles_n;
+    const int band = r0 / per_band;
+    const int first_m = band * p.group_m;
+    const int height = min(count - first_m, p.group_m);
+    const int r = r0 - band * per_band;
+    o.slot = first + first_m + r % height;
+    o.m0 = (kWgrad ? 0 : o.lo) + (first_m + r % height) * GROUP_SLOT_ROWS;
+    o.bn = half < 0 ? pl.bn : pl.bn / 2;
+    o.n0 = (r / height) * pl.bn + (half > 0 ? pl.bn / 2 : 0);
+    return o;
+}
+
+// One 32-row band of a finished tile to C. `rows_end`: rows from here on are not this tile's. zero: the sum is empty.
+template <int DT, bool kWgrad>
+__device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensorMap &tmC, uint32_t tmem_band, const GroupedTile &t, int row0,
+                                             int rows_end, bool zero, uint32_t epi_smem, uint32_t &tile_count, int lane)
+{
+    if (row0 >= rows_end) return;
+    const int z = kWgrad ? t.g : 0;
+    const long long base = (long long)z * p.strideC;
+    if (!p.c_vec_ok) {
+        const int row = row0 + lane;
+#pragma unroll 1
+        for (int c = 0; c < t.bn / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32(tmem_band + (uint32_t)(c * 32), v);
+            tmem_ld_wait();
+            if (zero) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0u;
+            }
+            const int col = t.n0 + c * 32, valid = min(32, p.N - col);
+            if (row < rows_end && valid > 0) store_row_direct<DT>(p, v, base + (long long)row * p.ldc + col, valid);
+        }
+        return;
+    }
+    const uint32_t swz = (uint32_t)(lane & 7);
+    const bool whole = kWgrad || row0 + 32 <= rows_end; // C[g] is clipped by its tensor map
+#pragma unroll 1
+    for (int c = 0; c < t.bn / 64; ++c) {
+        const int col = t.n0 + c * 64;
+        if (col >= p.N) break;
+        const uint32_t buf = epi_smem + (tile_count & 1u) * EPI_TILE_BYTES;
+        ++tile_count;
+        if (lane == 0) bulk_wait_read<1>();
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t v[32], q[16];
+            tmem_ld_32x32(tmem_band + (uint32_t)(c * 64 + h * 32), v);
+            tmem_ld_wait();
+            pack16<DT>(v, q);
+            if (zero) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) q[j] = 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                st_shared_v4(buf + (uint32_t)lane * 128u + (((uint32_t)(h * 4 + j) ^ swz) << 4), q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
+        }
+        if (whole) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_3d(&tmC, buf, col, row0, z);
+                bulk_commit();
+            }
+        } else {
+            __syncwarp();
+            uint16_t *dst = reinterpret_cast<uint16_t *>(p.C[0]);
+            const int j = lane & 7, ccol = col + j * 8;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3), row = row0 + r;
+                if (row < rows_end && ccol < p.N) {
+                    uint4 v;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                 : "r"(buf + (uint32_t)r * 128u + (((uint32_t)(j ^ (r & 7))) << 4)));
+                    const long long off = base + (long long)row * p.ldc + ccol;
+                    if (store_in_bounds(p, off, min(8, p.N - ccol))) {
+                        if (ccol + 8 <= p.N) {
+                            *reinterpret_cast<uint4 *>(dst + off) = v;
+                        } else {
+                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (ccol + e < p.N) dst[off + e] = (uint16_t)((e & 1) ? (w[e >> 1] >> 16) : (w[e >> 1] & 0xFFFFu));
+                        }
+                    }
+                }
+            }
+            if (lane == 0) bulk_commit(); // an empty group keeps the buffer accounting uniform
+        }
+    }
+}
+
+} // namespace btm

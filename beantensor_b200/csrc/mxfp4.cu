@@ -1,4 +1,4 @@
-// Microscaled 4-bit operands: quantisation, its inverse and the product (format: mxfp4.cuh).
+// Microscaled 4-bit operands: quantisation and its inverse (format: mxfp4.cuh; the product is in mxfp4_tc.cu).
 //
 // Quantise: for a block of 32 values, X = floor(log2(max |x|)) - 2 (the largest E2M1 value is 1.5 * 2^2), clamped to
 // [-127, 127], and q = x / 2^X rounded to nearest (ties to the even code) and saturated at 6. A division by a power of two
@@ -210,64 +210,6 @@ int launch_mxfp4_dequant(cudaStream_t st, int dst_dtype, int groups, int rows, i
     else if (dst_dtype == BTM_F16) mxfp4_dequant_kernel<__half><<<grid, mxq::THREADS, 0, st>>>(pk, sc, groups, rows, K, offsets, (__half *)out, ldo, vec, status);
     else mxfp4_dequant_kernel<__nv_bfloat16><<<grid, mxq::THREADS, 0, st>>>(pk, sc, groups, rows, K, offsets, (__nv_bfloat16 *)out, ldo, vec, status);
     return check_cuda(cudaGetLastError(), "mxfp4 dequantise launch");
-}
-
-// ---------------------------------------------------------------------------------------------------- product
-// First form: one thread per output, fp32 sums.
-template <typename T>
-__global__ void __launch_bounds__(256) mxfp4_matmul_simple_kernel(const Mxfp4Call c, int *status)
-{
-    const int chunks = mx_chunks(c.K);
-    const int slot = blockIdx.y >> 3; // 16 rows per block
-    GroupWalk walk;
-    int row0, row_end, g = 0, first_slot = 0, lo = 0;
-    if (c.offsets == nullptr) {
-        if (slot * GROUP_SLOT_ROWS >= c.rows) return;
-        row_end = c.rows;
-    } else {
-        walk.init(c.offsets, c.groups, c.rows);
-        const int total = walk.count_slots();
-        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 32) walk.report(status);
-        if (slot >= total) return;
-        walk.find_slot(slot, g, lo, row_end, first_slot);
-    }
-    const int r = (blockIdx.y & 7) * 16 + (threadIdx.x >> 4), n = blockIdx.x * 16 + (threadIdx.x & 15);
-    row0 = lo + (slot - first_slot) * GROUP_SLOT_ROWS;
-    const int row = row0 + r;
-    if (row >= row_end || n >= c.N) return;
-    const uint8_t *a = (const uint8_t *)c.act + (long long)row * (c.K / 2);
-    const uint8_t *w = (const uint8_t *)c.w + ((long long)g * c.N + n) * (c.K / 2);
-    const uint8_t *as = (const uint8_t *)c.act_scales + (long long)slot * chunks * MX_SCALE_BYTES;
-    const uint8_t *ws = (const uint8_t *)c.w_scales + ((long long)g * ((c.N + 127) / 128) + n / 128) * chunks * MX_SCALE_BYTES;
-    float sum = 0.0f;
-    for (int b = 0; b < c.K / MX_BLOCK; ++b) {
-        float part = 0.0f;
-        for (int j = 0; j < 4; ++j) {
-            uint32_t ah[4], wh[4];
-            mx_decode8(*reinterpret_cast<const uint32_t *>(a + b * 16 + j * 4), ah);
-            mx_decode8(*reinterpret_cast<const uint32_t *>(w + b * 16 + j * 4), wh);
-            for (int i = 0; i < 4; ++i) {
-                const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&ah[i])), y = __half22float2(*reinterpret_cast<const __half2 *>(&wh[i]));
-                part = fmaf(x.x, y.x, fmaf(x.y, y.y, part));
-            }
-        }
-        const int at = (b >> 2) * MX_SCALE_BYTES;
-        // The two exponents meet before they meet the sum, so that a large and a small scale do not overflow on the way.
-        const int sa = as[at + mx_scale_at(r, b & 3)], sw = ws[at + mx_scale_at(n & 127, b & 3)];
-        sum += (sa == (int)MX_NAN || sw == (int)MX_NAN) ? mx_scale_value(MX_NAN) : ldexpf(part, sa + sw - 254);
-    }
-    reinterpret_cast<T *>(c.out)[(long long)row * c.ldo + n] = round_to<T>(sum);
-}
-
-int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *status)
-{
-    (void)sm_count;
-    const long long slots = c.offsets ? grouped_slot_bound(c.groups, c.rows) : (c.rows + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS;
-    if (slots * 8 > 65535) return set_error(BTM_ERR_UNSUPPORTED, "mxfp4 matmul: too many rows");
-    const dim3 grid((unsigned)((c.N + 15) / 16), (unsigned)(slots * 8));
-    if (c.dtype == BTM_F16) mxfp4_matmul_simple_kernel<__half><<<grid, 256, 0, st>>>(c, status);
-    else mxfp4_matmul_simple_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(c, status);
-    return check_cuda(cudaGetLastError(), "mxfp4 matmul launch");
 }
 
 } // namespace btm
