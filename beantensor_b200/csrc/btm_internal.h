@@ -114,6 +114,9 @@ struct GroupedCall {
     long long ldc, strideC;
 };
 int configure_gemm_grouped_kernels();
+int configure_gemm_grouped_pair_kernels();
+int launch_gemm_grouped_pair(const GroupedCall &c, cudaStream_t st, int sm_count, const CUtensorMap &tmA, const CUtensorMap &tmA_band,
+                             const CUtensorMap &tmB, const CUtensorMap &tmC, GemmParams p);
 int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int *status);
 long long grouped_slot_bound(int groups, int rows);
 // Microscaled 4-bit operands (mxfp4.cu). offsets == NULL: every group has rows / groups rows.

@@ -20,6 +20,7 @@
 //
 // General kernel (operands that TMA cannot address, K == 0): 64 x 64 output tiles on CUDA cores as in gemm_simt.cu, fp32
 // accumulation, one rounding. A block finds its group by walking the table.
+#include <cstdlib>
 #include <cstring>
 
 #include <cuda_bf16.h>
@@ -31,8 +32,6 @@
 #include "grouped_tile.cuh"
 
 namespace btm {
-
-enum GroupedMode { GROUPED_KN = 0 /* B[g] is [K, N] */, GROUPED_NK = 1 /* B[g] is [N, K] */, GROUPED_WGRAD = 2 };
 
 namespace gg {
 constexpr int BM = 128;                 // rows of an output tile = accumulator lanes
@@ -92,7 +91,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    GroupWalk walk;
+    GroupWalk<> walk;
     walk.init(tab.offsets, tab.groups, tab.rows);
     const int group_slots = walk.count_slots();
     if (blockIdx.x == 0 && warp == 0) walk.report(p.status);
@@ -280,7 +279,7 @@ __global__ void __launch_bounds__(256) gemm_grouped_simt_kernel(const GroupedSim
     constexpr int TM = 64, TN = 64, TK = 16;
     __shared__ float As[TK][TM + 1];
     __shared__ float Bs[TK][TN + 1];
-    GroupWalk walk;
+    GroupWalk<> walk;
     walk.init(p.offsets, p.groups, p.rows);
     const long long id = blockIdx.x;
     const int n0 = (int)(id % p.tiles_n) * TN;
@@ -476,6 +475,15 @@ int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int
         rc = encode_tmap_3d(&tmC, c.dtype, c.C, (uint64_t)c.N, (uint64_t)p.M, (uint64_t)p.batch, pc, p.batch > 1 ? (uint64_t)c.strideC * 2 : pc, 64, 32);
         if (rc) return rc;
     }
+    // Pairs of CTAs when the groups are tall and deep enough. BTM_FORCE_KERNEL=1cta|2cta as for the dense products.
+    const long long pair_slots = c.wgrad ? (long long)c.groups * ((c.M + 255) / 256) : c.rows / 256;
+    bool pair = c.wgrad ? c.M > 128 && c.rows / c.groups >= 512 : c.rows / c.groups >= 512 && c.K >= 512;
+    pair = pair && pair_slots * ((c.N + 255) / 256) >= sm_count / 4;
+    if (const char *force = getenv("BTM_FORCE_KERNEL")) {
+        if (!strcmp(force, "1cta")) pair = false;
+        else if (!strcmp(force, "2cta")) pair = true;
+    }
+    if (pair) return launch_gemm_grouped_pair(c, st, sm_count, tmA, tmA_band, tmB, tmC, p);
     const int grid = (int)(most < sm_count ? most : sm_count);
 #define BTM_GROUPED_CASE(DT)                                                                                    \
     do {                                                                                                        \

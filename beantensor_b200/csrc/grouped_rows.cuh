@@ -11,9 +11,11 @@
 
 namespace btm {
 
-constexpr int GROUP_SLOT_ROWS = 128; // a group's rows are cut into slots of this many rows, the last one short
+constexpr int GROUP_SLOT_ROWS = 128; // a group's rows are cut into slots, the last one short: of so many rows, or twice
+                                     // as many for a pair of CTAs
 
 // All members are used by a whole warp at once. Without a table there is one group that owns every row.
+template <int kSlot = GROUP_SLOT_ROWS>
 struct GroupWalk {
     const int *offsets;
     int groups, rows;
@@ -39,7 +41,7 @@ struct GroupWalk {
         bad |= first + lane < groups && raw != hi ? 1 : 0;
         lo = __shfl_up_sync(0xffffffffu, hi, 1);
         if (lane == 0) lo = floor_at;
-        incl = (hi - lo + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS;
+        incl = (hi - lo + kSlot - 1) / kSlot;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int o = __shfl_up_sync(0xffffffffu, incl, d);
@@ -80,7 +82,7 @@ struct GroupWalk {
         group = g0 + l;
         row_lo = __shfl_sync(0xffffffffu, lo, l);
         row_hi = __shfl_sync(0xffffffffu, hi, l);
-        first_slot = slots_before + __shfl_sync(0xffffffffu, incl, l) - (row_hi - row_lo + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS;
+        first_slot = slots_before + __shfl_sync(0xffffffffu, incl, l) - (row_hi - row_lo + kSlot - 1) / kSlot;
     }
     // The rows of `group`, which must not be below that of an earlier call.
     __device__ __forceinline__ void find_group(int group, int &row_lo, int &row_hi)

@@ -7,6 +7,8 @@
 
 namespace btm {
 
+enum GroupedMode { GROUPED_KN = 0 /* B[g] is [K, N] */, GROUPED_NK = 1 /* B[g] is [N, K] */, GROUPED_WGRAD = 2 };
+
 struct GroupedTables {
     const int *offsets;
     int groups, rows;
@@ -20,18 +22,18 @@ struct GroupedPlan {
 
 // Cost of a tile in units of B columns: its columns plus kTileOverhead for what does not shrink with the width (the A
 // rows, the hand-offs). Waves are counted whole, a last one that fits twice over is run as half-width tiles.
-template <int kWidest>
+template <int kWidest, int kNarrowest = 64>
 __device__ __forceinline__ GroupedPlan plan_tiles(int slots, int N, int ctas)
 {
     constexpr int kTileOverhead = 64;
     GroupedPlan best;
     long long best_cost = 0x7FFFFFFFFFFFFFFFLL;
 #pragma unroll
-    for (int bn = kWidest; bn >= 64; bn = bn > 128 ? 128 : bn / 2) {
+    for (int bn = kWidest; bn >= kNarrowest; bn = bn > 128 ? 128 : bn / 2) {
         const int tiles_n = (N + bn - 1) / bn;
         const int tiles = slots * tiles_n;
         const int waves = tiles / ctas, rem = tiles - waves * ctas;
-        const bool halves = bn % 128 == 0 && rem > 0 && 2 * rem <= ctas;
+        const bool halves = bn % 128 == 0 && bn / 2 >= kNarrowest && rem > 0 && 2 * rem <= ctas;
         const long long cost = (long long)waves * (bn + kTileOverhead) + (rem == 0 ? 0 : (halves ? bn / 2 : bn) + kTileOverhead);
         if (cost < best_cost) {
             best_cost = cost;
@@ -51,8 +53,8 @@ struct GroupedTile {
     int n0, bn;    // columns
 };
 
-template <bool kWgrad>
-__device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const GroupedPlan &pl, GroupWalk &walk, int t)
+template <bool kWgrad, int kSlot>
+__device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const GroupedPlan &pl, GroupWalk<kSlot> &walk, int t)
 {
     GroupedTile o;
     int tile = t, half = -1;
@@ -70,7 +72,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const G
         walk.find_group(o.g, o.lo, o.hi);
     } else {
         walk.find_slot(slot, o.g, o.lo, o.hi, first);
-        count = (o.hi - o.lo + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS;
+        count = (o.hi - o.lo + kSlot - 1) / kSlot;
     }
     // Within a group: bands of group_m row tiles, row tiles innermost, so that neighbouring CTAs share columns of B.
     const int r0 = tile - first * pl.tiles_n;
@@ -80,7 +82,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const G
     const int height = min(count - first_m, p.group_m);
     const int r = r0 - band * per_band;
     o.slot = first + first_m + r % height;
-    o.m0 = (kWgrad ? 0 : o.lo) + (first_m + r % height) * GROUP_SLOT_ROWS;
+    o.m0 = (kWgrad ? 0 : o.lo) + (first_m + r % height) * kSlot;
     o.bn = half < 0 ? pl.bn : pl.bn / 2;
     o.n0 = (r / height) * pl.bn + (half > 0 ? pl.bn / 2 : 0);
     return o;

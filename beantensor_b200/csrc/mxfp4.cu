@@ -32,7 +32,7 @@ __device__ __forceinline__ bool slot_rows(int slot, const int *offsets, int grou
         row0 = g * per + m * GROUP_SLOT_ROWS;
         row_end = (g + 1) * per;
     } else {
-        GroupWalk walk;
+        GroupWalk<> walk;
         walk.init(offsets, groups, rows);
         const int total = walk.count_slots();
         if (blockIdx.x == 0 && threadIdx.x < 32) walk.report(status);

@@ -84,7 +84,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    GroupWalk walk;
+    GroupWalk<> walk;
     walk.init(op.offsets, op.groups, op.rows);
     const GroupedPlan plan = plan_tiles<BN>(walk.count_slots(), p.N, gridDim.x);
     if (blockIdx.x == 0 && warp == 0) walk.report(p.status);

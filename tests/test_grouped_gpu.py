@@ -33,6 +33,12 @@ def table(bounds):
     return torch.tensor(bounds, dtype=torch.int32, device="cuda")
 
 
+@pytest.fixture(params=["1cta", "2cta"])
+def kernel(request, monkeypatch):
+    """Both tensor-core kernels on every shape; operands that they cannot address take the general one either way."""
+    monkeypatch.setenv("BTM_FORCE_KERNEL", request.param)
+
+
 def expect_product(a, b, bounds, rows, out, before):
     """out against the plain form; what no group owns has to be as before."""
     touched = torch.zeros(rows, dtype=torch.bool, device="cuda")
@@ -48,7 +54,7 @@ def expect_product(a, b, bounds, rows, out, before):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("name", TABLES)
 @pytest.mark.parametrize("K,N", DENSE + ODD)
-def test_product(btm, name, dtype, K, N, trans):
+def test_product(btm, kernel, name, dtype, K, N, trans):
     bounds, rows = TABLES[name]
     a = normal((rows, K), dtype, 1)
     groups = len(bounds) - 1
@@ -63,7 +69,7 @@ def test_product(btm, name, dtype, K, N, trans):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("name", TABLES)
 @pytest.mark.parametrize("K,N", DENSE + ODD)
-def test_wgrad(btm, name, dtype, K, N):
+def test_wgrad(btm, kernel, name, dtype, K, N):
     bounds, rows = TABLES[name]
     a, d = normal((rows, K), dtype, 1), normal((rows, N), dtype, 2)
     out = normal((len(bounds) - 1, K, N), dtype, 3)
@@ -75,7 +81,7 @@ def test_wgrad(btm, name, dtype, K, N):
 
 
 @pytest.mark.parametrize("rows,groups,K,N", [(1500, 3, 1024, 2048), (4100, 9, 776, 1544), (300, 130, 256, 512)])
-def test_larger_products_and_gradients(btm, rows, groups, K, N):
+def test_larger_products_and_gradients(btm, kernel, rows, groups, K, N):
     g = torch.Generator().manual_seed(rows)
     cuts = sorted(torch.randint(0, rows + 1, (groups - 1,), generator=g).tolist())
     bounds = [0] + cuts + [rows]
@@ -94,7 +100,7 @@ def test_larger_products_and_gradients(btm, rows, groups, K, N):
         ragged.check(db[i], exact, mass, hi - lo)
 
 
-def test_gradients_against_differences(btm):
+def test_gradients_against_differences(btm, kernel):
     # L = sum(out * d) is linear in a and in b: L(x + step) - L(x - step) is <gradient, 2 step> but for the roundings of the
     # outputs and of the gradient, each within its bound.
     bounds, rows, K, N = [0, 33, 33, 170, 201], 201, 136, 72
@@ -126,7 +132,7 @@ def test_gradients_against_differences(btm):
         assert (lp - lm - want).abs() <= op + om + (lim * real.abs()).sum()
 
 
-def test_foreign_rows_never_enter(btm):
+def test_foreign_rows_never_enter(btm, kernel):
     # Infinities and NaN in rows of other groups, behind the last group and in front of the first one.
     bounds, rows, K, N = [3, 20, 41, 41, 200], 230, 200, 136
     for dtype in (F16, BF16):
@@ -151,7 +157,7 @@ def test_foreign_rows_never_enter(btm):
 
 
 @pytest.mark.parametrize("pad", [0, 8, 3])
-def test_strided_operands(btm, pad):
+def test_strided_operands(btm, kernel, pad):
     # Column ranges of wider buffers, groups of b apart from each other, an output inside a wider one whose rest is kept.
     bounds, rows, K, N = [0, 50, 179, 260], 260, 128, 200
     a_all, b_all, c_all = normal((rows, K + pad), F16, 1), normal((3, K + 5, N + pad), F16, 2), normal((rows, N + 2 * pad), F16, 3)
@@ -173,7 +179,7 @@ def test_strided_operands(btm, pad):
     assert torch.equal(w_all[:, K:], before[:, K:]) and torch.equal(w_all[:, :, pad + N:], before[:, :, pad + N:])
 
 
-def test_empty_calls(btm):
+def test_empty_calls(btm, kernel):
     e = torch.empty((0, 64), dtype=F16, device="cuda")
     b = normal((2, 64, 32), F16, 1)
     btm.grouped_matmul_gpu(e, b, table([0, 0, 0]), torch.empty((0, 32), dtype=F16, device="cuda"))
@@ -191,7 +197,7 @@ def test_empty_calls(btm):
 
 @pytest.mark.parametrize("bounds", [[0, 50, 20, 60], [0, 70, 500, 600], [-5, 10, 20, 60], [90, 80, 70, 60], [2 ** 31 - 1, -2 ** 31, 0, 2 ** 31 - 1]])
 @pytest.mark.parametrize("K,N", [(64, 72), (33, 21)])
-def test_bad_offsets_are_clamped_and_reported(btm, bounds, K, N):
+def test_bad_offsets_are_clamped_and_reported(btm, kernel, bounds, K, N):
     rows = 75
     a, d = normal((rows, K), BF16, 1), normal((rows, N), BF16, 4)
     b = normal((3, K, N), BF16, 2)
@@ -211,7 +217,7 @@ def test_bad_offsets_are_clamped_and_reported(btm, bounds, K, N):
         ragged.check(db[g], exact, mass, hi - lo)
 
 
-def test_captured_and_replayed_with_another_table(btm):
+def test_captured_and_replayed_with_another_table(btm, kernel):
     rows, K, N = 300, 192, 264
     a, d, b = normal((rows, K), BF16, 1), normal((rows, N), BF16, 2), normal((4, K, N), BF16, 3)
     out, da, db = torch.zeros_like(d), torch.zeros_like(a), torch.zeros_like(b)
@@ -240,7 +246,7 @@ def test_captured_and_replayed_with_another_table(btm):
             ragged.check(db[g], exact, mass, hi - lo)
 
 
-def test_two_streams_and_repeated_calls_give_the_same_bits(btm):
+def test_two_streams_and_repeated_calls_give_the_same_bits(btm, kernel):
     rows, K, N = 700, 520, 776
     a, b = normal((rows, K), F16, 1), normal((6, K, N), F16, 2)
     t = table([0, 3, 300, 301, 500, 500, 699])
@@ -261,7 +267,7 @@ def test_two_streams_and_repeated_calls_give_the_same_bits(btm):
             assert torch.equal(x, first)
 
 
-def test_chain_behind_the_router(btm):
+def test_chain_behind_the_router(btm, kernel):
     # The table and the rows come from work queued just before, the products feed one another back to back.
     tokens, groups, K, H = 200, 8, 256, 384
     x = normal((tokens, K), BF16, 1)
