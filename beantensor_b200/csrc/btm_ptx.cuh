@@ -161,6 +161,30 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// The wait for a warp that then issues tcgen05 or TMA instructions: all lanes poll and vote, so that control flow stays
+// uniform in the compiler's eyes and what the issue needs (descriptors, coordinates) can live in uniform registers. Moved there
+// one by one from a single-lane branch they cost the issuing warp about 100 cycles per tcgen05.mma instead of 36.
+template <bool kCluster = false>
+__device__ __forceinline__ bool mbar_wait_uniform(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code, long long limit_cycles)
+{
+    if (__all_sync(0xffffffffu, kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) return true;
+    const long long t0 = clock64();
+    while (true) {
+        if (__all_sync(0xffffffffu, kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) return true;
+        const bool late = clock64() - t0 > limit_cycles;
+        if (__any_sync(0xffffffffu, late || *abort_flag != 0)) {
+            if ((threadIdx.x & 31) == 0 && *abort_flag == 0) {
+                *abort_flag = 1;
+                atomicCAS(status, 0, code);
+            }
+            return false;
+        }
+    }
+}
+// A value that is the same in all lanes, into a uniform register.
+__device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *m)
 {

@@ -97,23 +97,23 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (blockIdx.x == 0 && warp == 0) walk.report(p.status);
     const GroupedPlan plan = plan_tiles<gg::BN>(kWgrad ? tab.groups * p.tiles_m : group_slots, p.N, gridDim.x);
 
+    // Producer and issuer run as whole warps with uniform control flow; one elected lane issues (mbar_wait_uniform).
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
         int stage = 0;
         uint32_t phase = 0;
         bool ok = !p.debug_skip_loads;
         for (int tile = blockIdx.x; ok && tile < plan.total; tile += gridDim.x) {
-            const GroupedTile t = grouped_tile<kWgrad>(p, plan, walk, tile);
+            const GroupedTile t = grouped_tile_uniform<kWgrad, GROUP_SLOT_ROWS>(p, plan, walk, tile);
             const int num_kb = kWgrad ? (t.hi - t.lo + BK - 1) / BK : p.num_kb;
             const int chunks = t.bn / 64;
             const int bands = min(4, (t.hi - t.m0 + A_BAND - 1) / A_BAND); // of A rows that the tile owns (product)
             const uint32_t bytes = (uint32_t)((kWgrad || bands == 4 ? A_BYTES : bands * A_BAND * 128) + chunks * CHUNK_BYTES);
-            // One lane runs the k-loop; the warp meets again for the next tile. (A warp that shuffles the outcome of every
-            // wait puts that latency into each turn of the ring.)
-            if (lane == 0) {
-                for (int kb = 0; kb < num_kb; ++kb) {
-                    ok = mbar_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
-                    if (!ok) break;
+            const int zb = kWgrad ? 0 : t.g;
+            for (int kb = 0; kb < num_kb; ++kb) {
+                ok = mbar_wait_uniform(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
+                if (!ok) break;
+                if (elect_one()) {
                     const uint32_t full = smem_u32(&bar_full[stage]);
                     const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
                     const int k0 = kWgrad ? t.lo + kb * BK : kb * BK;
@@ -126,86 +126,75 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     } else {
                         for (int b = 0; b < bands; ++b) tma_load_3d(a0 + b * A_BAND * 128, &tmA_band, k0, t.m0 + b * A_BAND, 0, full);
                     }
-                    const int zb = kWgrad ? 0 : t.g;
-                    for (int c = 0; c < chunks; ++c) {
-                        if (kBMnMajor) tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, t.n0 + c * 64, k0, zb, full);
-                        else tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, k0, t.n0 + c * 64, zb, full);
-                    }
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
+#pragma unroll
+                    for (int c = 0; c < BN / 64; ++c) {
+                        if (c < chunks) {
+                            if (kBMnMajor) tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, t.n0 + c * 64, k0, zb, full);
+                            else tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, k0, t.n0 + c * 64, zb, full);
+                        }
                     }
                 }
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
             }
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
         constexpr uint32_t kFmt = DT == BTM_BF16 ? 1u : 0u;
         constexpr uint32_t a_step = (kWgrad ? 16 * 128 : 32) >> 4, b_step = (kBMnMajor ? 16 * 128 : 32) >> 4; // 16 k, in 16-byte units
+        const uint32_t tmem_u = uniform(tmem_base);
         int stage = 0, it = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < plan.total; tile += gridDim.x, ++it) {
-            const GroupedTile t = grouped_tile<kWgrad>(p, plan, walk, tile);
+            const GroupedTile t = grouped_tile_uniform<kWgrad, GROUP_SLOT_ROWS>(p, plan, walk, tile);
             const int num_kb = kWgrad ? (t.hi - t.lo + BK - 1) / BK : p.num_kb;
             const uint32_t idesc = make_idesc(kFmt, kWgrad, kBMnMajor, BM, (uint32_t)t.bn);
             const int acc = it & 1;
-            ok = mbar_wait_warp(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
+            ok = mbar_wait_uniform(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-            int whole = num_kb; // k-blocks that need nothing but their MMAs
-            if (kWgrad && ((t.hi - t.lo) & (BK - 1)) != 0) --whole;
-            int kb = 0;
-            if (lane == 0) {
-                for (; kb < whole; ++kb) {
-                    ok = mbar_wait(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
-                    const uint64_t ad = kWgrad ? make_smem_desc_sw128(a0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(a0, 16, 1024);
-                    const uint64_t bd = kBMnMajor ? make_smem_desc_sw128(b0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(b0, 16, 1024);
+            const uint32_t d_tmem = tmem_u + (uint32_t)(acc * BN);
+            for (int kb = 0; kb < num_kb; ++kb) {
+                ok = mbar_wait_uniform(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
+                if (!ok) break;
+                const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
+                int steps = BK / 16;
+                if (kWgrad) {
+                    const int left = t.hi - t.lo - kb * BK; // rows of the group in this k-block
+                    if (left < BK) {
+                        steps = (left + 15) / 16;
+                        // Rows left .. 16 * steps - 1 of every 64-wide chunk: 128 contiguous bytes per row.
+                        const int dirty = steps * 16 - left;
+                        for (int i = lane; i < dirty * 8; i += 32) {
+                            const uint32_t off = (uint32_t)(left + (i >> 3)) * 128u + (uint32_t)(i & 7) * 16u;
+                            for (int c = 0; c < BM / 64; ++c) st_shared_v4(a0 + c * CHUNK_BYTES + off, 0u, 0u, 0u, 0u);
+                            for (int c = 0; c < t.bn / 64; ++c) st_shared_v4(b0 + c * CHUNK_BYTES + off, 0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
+                tc_fence_after();
+                const uint64_t ad = kWgrad ? make_smem_desc_sw128(a0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(a0, 16, 1024);
+                const uint64_t bd = kBMnMajor ? make_smem_desc_sw128(b0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(b0, 16, 1024);
+                if (elect_one()) {
 #pragma unroll
                     for (int ks = 0; ks < BK / 16; ++ks)
-                        umma<1, false>(d_tmem, ad + (uint64_t)(ks * a_step), bd + (uint64_t)(ks * b_step), idesc, (uint32_t)((kb | ks) != 0));
+                        if (!kWgrad || ks < steps)
+                            umma<1, false>(d_tmem, ad + (uint64_t)(ks * a_step), bd + (uint64_t)(ks * b_step), idesc, (uint32_t)((kb | ks) != 0));
                     umma_commit(smem_u32(&bar_empty[stage]));
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                }
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-            stage = __shfl_sync(0xffffffffu, stage, 0);
-            phase = __shfl_sync(0xffffffffu, phase, 0);
-            if (kWgrad && ok && whole < num_kb) {
-                ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
-                if (ok) {
-                    // Rows left .. 16 * steps - 1 of every 64-wide chunk: 128 contiguous bytes per row.
-                    const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
-                    const int left = (t.hi - t.lo) & (BK - 1), steps = (left + 15) / 16, dirty = steps * 16 - left;
-                    for (int i = lane; i < dirty * 8; i += 32) {
-                        const uint32_t off = (uint32_t)(left + (i >> 3)) * 128u + (uint32_t)(i & 7) * 16u;
-                        for (int c = 0; c < BM / 64; ++c) st_shared_v4(a0 + c * CHUNK_BYTES + off, 0u, 0u, 0u, 0u);
-                        for (int c = 0; c < t.bn / 64; ++c) st_shared_v4(b0 + c * CHUNK_BYTES + off, 0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint64_t ad = make_smem_desc_sw128(a0, CHUNK_BYTES, 1024), bd = make_smem_desc_sw128(b0, CHUNK_BYTES, 1024);
-                        for (int ks = 0; ks < steps; ++ks)
-                            umma<1, false>(d_tmem, ad + (uint64_t)(ks * a_step), bd + (uint64_t)(ks * b_step), idesc, (uint32_t)((whole | ks) != 0));
-                        umma_commit(smem_u32(&bar_empty[stage]));
-                    }
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                }
-            }
-            if (ok && lane == 0) umma_commit(smem_u32(&bar_tmem_full[acc]));
+            if (ok && elect_one()) umma_commit(smem_u32(&bar_tmem_full[acc]));
             __syncwarp();
         }
     } else {
@@ -215,7 +204,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         uint32_t epi_tiles = 0;
         int it = 0;
         for (int tile = blockIdx.x; tile < plan.total; tile += gridDim.x, ++it) {
-            const GroupedTile t = grouped_tile<kWgrad>(p, plan, walk, tile);
+            const GroupedTile t = grouped_tile<kWgrad, GROUP_SLOT_ROWS>(p, plan, walk, tile);
             const int acc = it & 1;
             if (!mbar_wait_warp(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();

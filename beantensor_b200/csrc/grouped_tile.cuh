@@ -43,6 +43,7 @@ __device__ __forceinline__ GroupedPlan plan_tiles(int slots, int N, int ctas)
             best.total = halves ? tiles + rem : tiles;
         }
     }
+    best.total = uniform(best.total);
     return best;
 }
 
@@ -85,6 +86,21 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const G
     o.m0 = (kWgrad ? 0 : o.lo) + (first_m + r % height) * kSlot;
     o.bn = half < 0 ? pl.bn : pl.bn / 2;
     o.n0 = (r / height) * pl.bn + (half > 0 ? pl.bn / 2 : 0);
+    return o;
+}
+
+// The same with every field in uniform registers, for the warps that issue TMA and tcgen05 instructions.
+template <bool kWgrad, int kSlot>
+__device__ __forceinline__ GroupedTile grouped_tile_uniform(const GemmParams &p, const GroupedPlan &pl, GroupWalk<kSlot> &walk, int t)
+{
+    GroupedTile o = grouped_tile<kWgrad, kSlot>(p, pl, walk, t);
+    o.g = uniform(o.g);
+    o.lo = uniform(o.lo);
+    o.hi = uniform(o.hi);
+    o.slot = uniform(o.slot);
+    o.m0 = uniform(o.m0);
+    o.n0 = uniform(o.n0);
+    o.bn = uniform(o.bn);
     return o;
 }
 
