@@ -114,117 +114,129 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     if (blockIdx.x == 0 && warp == 0) walk.report(p.status);
     const GroupedPlan plan = plan_tiles<BN, 128>(kWgrad ? tab.groups * p.tiles_m : group_slots, p.N, num_pairs);
 
+    // Producer and issuer run as whole warps with uniform control flow; one elected lane issues (mbar_wait_uniform).
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer (both CTAs)
         int stage = 0;
         uint32_t phase = 0;
         bool ok = !p.debug_skip_loads;
         for (int tile = pair_id; ok && tile < plan.total; tile += num_pairs) {
-            const GroupedTile t = grouped_tile<kWgrad, PAIR_M>(p, plan, walk, tile);
-            if (lane == 0) {
-                const int k_rows = t.hi - t.lo; // gradient: the reduction
-                const int num_kb = kWgrad ? k_rows / BK : p.num_kb;
-                const int half_bn = t.bn >> 1, chunks = half_bn >> 6;
-                const int am = t.m0 + (int)rank * CTA_M, bn0 = t.n0 + (int)rank * half_bn;
-                // 32-row bands of A that belong to the group, of this CTA and of the pair (product)
-                const int pair_bands = kWgrad ? 8 : min(4, (t.hi - t.m0 + A_BAND - 1) / A_BAND) + min(4, max(0, t.hi - t.m0 - CTA_M + A_BAND - 1) / A_BAND);
-                const int bands = kWgrad ? 4 : min(4, max(0, t.hi - am + A_BAND - 1) / A_BAND);
-                const uint32_t kb_bytes = (uint32_t)(pair_bands * A_BAND * 128 + 2 * chunks * CHUNK_BYTES);
-                const int zb = kWgrad ? 0 : t.g;
-                for (int kb = 0; kb < num_kb; kb += KPS) {
-                    ok = mbar_wait<true>(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
-                    if (!ok) break;
-                    const int nsub = min(KPS, num_kb - kb);
+            const GroupedTile t = grouped_tile_uniform<kWgrad, PAIR_M>(p, plan, walk, tile);
+            const int k_rows = t.hi - t.lo; // gradient: the reduction
+            const int num_kb = kWgrad ? k_rows / BK : p.num_kb;
+            const int half_bn = t.bn >> 1, chunks = half_bn >> 6;
+            const int am = t.m0 + (int)rank * CTA_M, bn0 = t.n0 + (int)rank * half_bn;
+            // 32-row bands of A that belong to the group, of this CTA and of the pair (product)
+            const int pair_bands = kWgrad ? 8 : min(4, (t.hi - t.m0 + A_BAND - 1) / A_BAND) + min(4, max(0, t.hi - t.m0 - CTA_M + A_BAND - 1) / A_BAND);
+            const int bands = kWgrad ? 4 : min(4, max(0, t.hi - am + A_BAND - 1) / A_BAND);
+            const uint32_t kb_bytes = (uint32_t)(pair_bands * A_BAND * 128 + 2 * chunks * CHUNK_BYTES);
+            const int zb = kWgrad ? 0 : t.g;
+            for (int kb = 0; kb < num_kb; kb += KPS) {
+                ok = mbar_wait_uniform<true>(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
+                if (!ok) break;
+                const int nsub = min(KPS, num_kb - kb);
+                if (elect_one()) {
                     const uint32_t full_local = smem_u32(&bar_full[stage]), full = map_to_leader(full_local);
                     if (rank == 0) mbar_expect_tx(full_local, kb_bytes * (uint32_t)nsub);
                     else if (kWgrad) mbar_arrive_cluster(full_local, 0);
-                    for (int sub = 0; sub < nsub; ++sub) {
-                        const uint32_t a0 = smem_base + stage * STAGE_BYTES + sub * KB_BYTES, b0 = a0 + A_BYTES;
-                        const int k0 = (kWgrad ? t.lo : 0) + (kb + sub) * BK;
-                        if constexpr (kWgrad) {
-                            tma_load_3d_2sm(a0, &tmA, am, k0, 0, full);
-                            tma_load_3d_2sm(a0 + CHUNK_BYTES, &tmA, am + 64, k0, 0, full);
-                        } else if (bands == 4) {
-                            tma_load_3d_2sm(a0, &tmA, k0, am, 0, full);
-                        } else {
-                            for (int b = 0; b < bands; ++b) tma_load_3d_2sm(a0 + b * A_BAND * 128, &tmA_band, k0, am + b * A_BAND, 0, full);
+#pragma unroll
+                    for (int sub = 0; sub < KPS; ++sub) {
+                        if (sub < nsub) {
+                            const uint32_t a0 = smem_base + stage * STAGE_BYTES + sub * KB_BYTES, b0 = a0 + A_BYTES;
+                            const int k0 = (kWgrad ? t.lo : 0) + (kb + sub) * BK;
+                            if constexpr (kWgrad) {
+                                tma_load_3d_2sm(a0, &tmA, am, k0, 0, full);
+                                tma_load_3d_2sm(a0 + CHUNK_BYTES, &tmA, am + 64, k0, 0, full);
+                            } else if (bands == 4) {
+                                tma_load_3d_2sm(a0, &tmA, k0, am, 0, full);
+                            } else {
+                                for (int b = 0; b < bands; ++b) tma_load_3d_2sm(a0 + b * A_BAND * 128, &tmA_band, k0, am + b * A_BAND, 0, full);
+                            }
+#pragma unroll
+                            for (int c = 0; c < BN / 128; ++c) {
+                                if (c < chunks) {
+                                    if (kBMnMajor) tma_load_3d_2sm(b0 + c * CHUNK_BYTES, &tmB, bn0 + c * 64, k0, zb, full);
+                                    else tma_load_3d_2sm(b0 + c * CHUNK_BYTES, &tmB, k0, bn0 + c * 64, zb, full);
+                                }
+                            }
                         }
-                        for (int c = 0; c < chunks; ++c) {
-                            if (kBMnMajor) tma_load_3d_2sm(b0 + c * CHUNK_BYTES, &tmB, bn0 + c * 64, k0, zb, full);
-                            else tma_load_3d_2sm(b0 + c * CHUNK_BYTES, &tmB, k0, bn0 + c * 64, zb, full);
-                        }
-                    }
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
                     }
                 }
-                if (kWgrad && ok && (k_rows & (BK - 1)) != 0) {
-                    ok = mbar_wait<true>(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
-                    if (ok) {
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (kWgrad && ok && (k_rows & (BK - 1)) != 0) {
+                ok = mbar_wait_uniform<true>(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
+                if (ok) {
+                    if (elect_one()) {
                         const uint32_t cut = smem_u32(&bar_cut[stage]), a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
                         const int k0 = t.lo + num_kb * BK;
                         mbar_expect_tx(cut, (uint32_t)(A_BYTES + chunks * CHUNK_BYTES));
                         tma_load_3d(a0, &tmA, am, k0, 0, cut);
                         tma_load_3d(a0 + CHUNK_BYTES, &tmA, am + 64, k0, 0, cut);
                         for (int c = 0; c < chunks; ++c) tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, bn0 + c * 64, k0, 0, cut);
-                        if (++stage == STAGES) {
-                            stage = 0;
-                            phase ^= 1u;
-                        }
+                    }
+                    __syncwarp();
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
                     }
                 }
             }
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         }
     } else if (warp == 1 && (rank == 0 || kWgrad)) {
         // ------------------------------------------------------------ MMA issuer (leader), zeroing of cut k-blocks (both)
         constexpr uint32_t kFmt = DT == BTM_BF16 ? 1u : 0u;
         constexpr uint32_t a_step = (kWgrad ? 16 * 128 : 32) >> 4, b_step = (kBMnMajor ? 16 * 128 : 32) >> 4;
+        const uint32_t tmem_u = uniform(tmem_base);
         int stage = 0, it = 0;
         uint32_t phase = 0, cut_phases = 0; // cut_phases: one bit per stage
         bool ok = true;
         for (int tile = pair_id; ok && tile < plan.total; tile += num_pairs, ++it) {
-            const GroupedTile t = grouped_tile<kWgrad, PAIR_M>(p, plan, walk, tile);
+            const GroupedTile t = grouped_tile_uniform<kWgrad, PAIR_M>(p, plan, walk, tile);
             const int k_rows = t.hi - t.lo;
             const int num_kb = kWgrad ? k_rows / BK : p.num_kb;
             const int left = kWgrad ? k_rows & (BK - 1) : 0; // rows of the cut k-block
             const uint32_t idesc = make_idesc(kFmt, kWgrad, kBMnMajor, PAIR_M, (uint32_t)t.bn);
             const int acc = it & 1;
-            const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+            const uint32_t d_tmem = tmem_u + (uint32_t)(acc * BN);
             if (rank == 0) {
-                if (lane == 0) {
-                    ok = mbar_wait<true>(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
+                ok = mbar_wait_uniform<true>(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
+                tc_fence_after();
+                for (int kb = 0; ok && kb < num_kb; kb += KPS) {
+                    ok = mbar_wait_uniform<true>(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
+                    if (!ok) break;
                     tc_fence_after();
-                    for (int kb = 0; ok && kb < num_kb; kb += KPS) {
-                        ok = mbar_wait<true>(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const int nsub = min(KPS, num_kb - kb);
-                        const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
-                        const uint64_t ad = kWgrad ? make_smem_desc_sw128(a0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(a0, 16, 1024);
-                        const uint64_t bd = kBMnMajor ? make_smem_desc_sw128(b0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(b0, 16, 1024);
-                        for (int sub = 0; sub < nsub; ++sub) {
+                    const int nsub = min(KPS, num_kb - kb);
+                    const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
+                    const uint64_t ad = kWgrad ? make_smem_desc_sw128(a0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(a0, 16, 1024);
+                    const uint64_t bd = kBMnMajor ? make_smem_desc_sw128(b0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(b0, 16, 1024);
+                    if (elect_one()) {
 #pragma unroll
-                            for (int ks = 0; ks < BK / 16; ++ks)
-                                umma<2, false>(d_tmem, ad + (uint64_t)((sub * KB_BYTES >> 4) + ks * a_step), bd + (uint64_t)((sub * KB_BYTES >> 4) + ks * b_step),
-                                               idesc, (uint32_t)((kb | sub | ks) != 0));
+                        for (int sub = 0; sub < KPS; ++sub) {
+                            if (sub < nsub) {
+#pragma unroll
+                                for (int ks = 0; ks < BK / 16; ++ks)
+                                    umma<2, false>(d_tmem, ad + (uint64_t)((sub * KB_BYTES >> 4) + ks * a_step), bd + (uint64_t)((sub * KB_BYTES >> 4) + ks * b_step),
+                                                   idesc, (uint32_t)((kb | sub | ks) != 0));
+                            }
                         }
                         umma_commit_2sm(smem_u32(&bar_empty[stage]), (uint16_t)3);
-                        if (++stage == STAGES) {
-                            stage = 0;
-                            phase ^= 1u;
-                        }
+                    }
+                    __syncwarp();
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        phase ^= 1u;
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                stage = __shfl_sync(0xffffffffu, stage, 0);
-                phase = __shfl_sync(0xffffffffu, phase, 0);
             } else {
                 stage = (stage + (num_kb + KPS - 1) / KPS) % STAGES; // the whole k-blocks' stages are the leader's business
             }
             if (kWgrad && ok && left != 0) {
-                ok = mbar_wait_warp(smem_u32(&bar_cut[stage]), (cut_phases >> stage) & 1u, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
+                ok = mbar_wait_uniform(smem_u32(&bar_cut[stage]), (cut_phases >> stage) & 1u, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
                 cut_phases ^= 1u << stage;
                 if (ok) {
                     const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
@@ -237,19 +249,17 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(smem_u32(&bar_full[stage]), 0);
+                    __syncwarp();
                     if (rank == 0) {
-                        ok = true;
-                        if (lane == 0) {
-                            ok = mbar_wait<true>(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
-                            if (ok) {
-                                tc_fence_after();
-                                const uint64_t ad = make_smem_desc_sw128(a0, CHUNK_BYTES, 1024), bd = make_smem_desc_sw128(b0, CHUNK_BYTES, 1024);
-                                for (int ks = 0; ks < steps; ++ks)
-                                    umma<2, false>(d_tmem, ad + (uint64_t)(ks * a_step), bd + (uint64_t)(ks * b_step), idesc, (uint32_t)((num_kb | ks) != 0));
-                                umma_commit_2sm(smem_u32(&bar_empty[stage]), (uint16_t)3);
-                            }
+                        ok = mbar_wait_uniform<true>(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
+                        tc_fence_after();
+                        if (ok && elect_one()) {
+                            const uint64_t ad = make_smem_desc_sw128(a0, CHUNK_BYTES, 1024), bd = make_smem_desc_sw128(b0, CHUNK_BYTES, 1024);
+                            for (int ks = 0; ks < steps; ++ks)
+                                umma<2, false>(d_tmem, ad + (uint64_t)(ks * a_step), bd + (uint64_t)(ks * b_step), idesc, (uint32_t)((num_kb | ks) != 0));
+                            umma_commit_2sm(smem_u32(&bar_empty[stage]), (uint16_t)3);
                         }
-                        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                        __syncwarp();
                     }
                     if (++stage == STAGES) {
                         stage = 0;
@@ -257,7 +267,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                     }
                 }
             }
-            if (rank == 0 && ok && lane == 0) umma_commit_2sm(smem_u32(&bar_tmem_full[acc]), (uint16_t)3);
+            if (rank == 0 && ok && elect_one()) umma_commit_2sm(smem_u32(&bar_tmem_full[acc]), (uint16_t)3);
             __syncwarp();
         }
     } else if (warp >= 2) {

@@ -96,7 +96,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         uint32_t phase = 0;
         bool ok = !p.debug_skip_loads;
         for (int tile = blockIdx.x; ok && tile < plan.total; tile += gridDim.x) {
-            const GroupedTile t = grouped_tile<false>(p, plan, walk, tile);
+            const GroupedTile t = grouped_tile_uniform<false, GROUP_SLOT_ROWS>(p, plan, walk, tile);
             const int bands = min(4, (t.hi - t.m0 + A_BAND - 1) / A_BAND);
             const int chunks = t.bn / 64;
             const int nb0 = t.n0 / 128;
@@ -104,9 +104,9 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             const uint8_t *sfa = op.act_scales + (long long)t.slot * k_chunks * MX_SCALE_BYTES;
             const uint8_t *sfb = op.w_scales + ((long long)t.g * n_blocks + nb0) * k_chunks * MX_SCALE_BYTES;
             for (int kb = 0; kb < p.num_kb; ++kb) {
-                ok = mbar_wait_warp(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
+                ok = mbar_wait_uniform(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
                 if (!ok) break;
-                if (lane == 0) {
+                if (elect_one()) {
                     const uint32_t full = smem_u32(&bar_full[stage]);
                     const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
                     const uint32_t sf_bytes = (uint32_t)min(2, k_chunks - kb * 2) * MX_SCALE_BYTES;
@@ -116,11 +116,14 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                     } else {
                         for (int b = 0; b < bands; ++b) tma_load_3d(a0 + b * A_BAND * 128, &tmA_band, kb * 128, t.m0 + b * A_BAND, 0, full);
                     }
-                    for (int c = 0; c < chunks; ++c) tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, kb * 128, t.n0 + c * 64, t.g, full);
+#pragma unroll
+                    for (int c = 0; c < BN / 64; ++c)
+                        if (c < chunks) tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, kb * 128, t.n0 + c * 64, t.g, full);
                     bulk_load(a0 + SFA_AT, sfa + kb * 2 * MX_SCALE_BYTES, sf_bytes, full);
                     for (int b = 0; b < nb; ++b)
                         bulk_load(a0 + SFB_AT + b * 2 * MX_SCALE_BYTES, sfb + ((long long)b * k_chunks + kb * 2) * MX_SCALE_BYTES, sf_bytes, full);
                 }
+                __syncwarp();
                 if (++stage == STAGES) {
                     stage = 0;
                     phase ^= 1u;
@@ -129,26 +132,27 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
+        const uint32_t tmem_u = uniform(tmem_base);
         int stage = 0, it = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < plan.total; tile += gridDim.x, ++it) {
-            const GroupedTile t = grouped_tile<false>(p, plan, walk, tile);
+            const GroupedTile t = grouped_tile_uniform<false, GROUP_SLOT_ROWS>(p, plan, walk, tile);
             const uint32_t idesc[2] = {make_idesc_mxf4(BM, (uint32_t)t.bn, 0), make_idesc_mxf4(BM, (uint32_t)t.bn, 2)};
             const uint32_t n_skip = (uint32_t)(t.n0 & 127) >> 5; // a tile may start in the middle of a row block: two columns in
             const int acc = it & 1;
-            ok = mbar_wait_warp(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
+            ok = mbar_wait_uniform(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+            const uint32_t d_tmem = tmem_u + (uint32_t)(acc * BN);
             for (int kb = 0; kb < p.num_kb; ++kb) {
-                ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
+                ok = mbar_wait_uniform(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t a0 = smem_base + stage * STAGE_BYTES;
                 const uint64_t ad = make_smem_desc_sw128(a0, 16, 1024), bd = make_smem_desc_sw128(a0 + A_BYTES, 16, 1024);
                 const uint64_t sa = make_smem_desc_rows16(a0 + SFA_AT), sb = make_smem_desc_rows16(a0 + SFB_AT);
-                const uint32_t sf = tmem_base + SF_COL + (uint32_t)(stage * SF_STAGE_COLS);
+                const uint32_t sf = tmem_u + SF_COL + (uint32_t)(stage * SF_STAGE_COLS);
                 const int steps = min(BK / 64, (p.K - kb * BK + 63) / 64);
                 if (elect_one()) {
 #pragma unroll
@@ -182,7 +186,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         uint32_t epi_tiles = 0;
         int it = 0;
         for (int tile = blockIdx.x; tile < plan.total; tile += gridDim.x, ++it) {
-            const GroupedTile t = grouped_tile<false>(p, plan, walk, tile);
+            const GroupedTile t = grouped_tile<false, GROUP_SLOT_ROWS>(p, plan, walk, tile);
             const int acc = it & 1;
             if (!mbar_wait_warp(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();
