@@ -72,6 +72,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     __shared__ __align__(8) uint64_t bar_empty[STAGES];  // per CTA
     __shared__ __align__(8) uint64_t bar_tmem_full[2];   // per CTA
     __shared__ __align__(8) uint64_t bar_tmem_empty[2];  // used in the leader
+    __shared__ __align__(8) uint64_t bar_clean[STAGES];  // used in the leader: both CTAs have zeroed it
     __shared__ __align__(8) uint64_t bar_cut[STAGES];    // per CTA: the cut k-block in this stage has landed (gradient)
     __shared__ uint32_t tmem_base_holder;
     __shared__ int abort_flag;
@@ -83,7 +84,8 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(smem_u32(&bar_full[s]), kWgrad ? 2 : 1);
+            mbar_init(smem_u32(&bar_full[s]), 1);
+            mbar_init(smem_u32(&bar_clean[s]), 2);
             mbar_init(smem_u32(&bar_empty[s]), 1);
             mbar_init(smem_u32(&bar_cut[s]), 1);
         }
@@ -138,7 +140,6 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                 if (elect_one()) {
                     const uint32_t full_local = smem_u32(&bar_full[stage]), full = map_to_leader(full_local);
                     if (rank == 0) mbar_expect_tx(full_local, kb_bytes * (uint32_t)nsub);
-                    else if (kWgrad) mbar_arrive_cluster(full_local, 0);
 #pragma unroll
                     for (int sub = 0; sub < KPS; ++sub) {
                         if (sub < nsub) {
@@ -193,7 +194,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         constexpr uint32_t a_step = (kWgrad ? 16 * 128 : 32) >> 4, b_step = (kBMnMajor ? 16 * 128 : 32) >> 4;
         const uint32_t tmem_u = uniform(tmem_base);
         int stage = 0, it = 0;
-        uint32_t phase = 0, cut_phases = 0; // cut_phases: one bit per stage
+        uint32_t full_phases = 0, cut_phases = 0; // one bit per stage
         bool ok = true;
         for (int tile = pair_id; ok && tile < plan.total; tile += num_pairs, ++it) {
             const GroupedTile t = grouped_tile_uniform<kWgrad, PAIR_M>(p, plan, walk, tile);
@@ -207,7 +208,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                 ok = mbar_wait_uniform<true>(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
                 tc_fence_after();
                 for (int kb = 0; ok && kb < num_kb; kb += KPS) {
-                    ok = mbar_wait_uniform<true>(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
+                    ok = mbar_wait_uniform<true>(smem_u32(&bar_full[stage]), (full_phases >> stage) & 1u, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
                     if (!ok) break;
                     tc_fence_after();
                     const int nsub = min(KPS, num_kb - kb);
@@ -227,17 +228,14 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                         umma_commit_2sm(smem_u32(&bar_empty[stage]), (uint16_t)3);
                     }
                     __syncwarp();
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                    full_phases ^= 1u << stage;
+                    if (++stage == STAGES) stage = 0;
                 }
             } else {
                 stage = (stage + (num_kb + KPS - 1) / KPS) % STAGES; // the whole k-blocks' stages are the leader's business
             }
             if (kWgrad && ok && left != 0) {
                 ok = mbar_wait_uniform(smem_u32(&bar_cut[stage]), (cut_phases >> stage) & 1u, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
-                cut_phases ^= 1u << stage;
                 if (ok) {
                     const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
                     const int steps = (left + 15) / 16, dirty = steps * 16 - left;
@@ -248,10 +246,10 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(smem_u32(&bar_full[stage]), 0);
+                    if (lane == 0) mbar_arrive_cluster(smem_u32(&bar_clean[stage]), 0);
                     __syncwarp();
                     if (rank == 0) {
-                        ok = mbar_wait_uniform<true>(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
+                        ok = mbar_wait_uniform<true>(smem_u32(&bar_clean[stage]), (cut_phases >> stage) & 1u, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
                         tc_fence_after();
                         if (ok && elect_one()) {
                             const uint64_t ad = make_smem_desc_sw128(a0, CHUNK_BYTES, 1024), bd = make_smem_desc_sw128(b0, CHUNK_BYTES, 1024);
@@ -261,10 +259,8 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                         }
                         __syncwarp();
                     }
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                    cut_phases ^= 1u << stage;
+                    if (++stage == STAGES) stage = 0;
                 }
             }
             if (rank == 0 && ok && elect_one()) umma_commit_2sm(smem_u32(&bar_tmem_full[acc]), (uint16_t)3);
