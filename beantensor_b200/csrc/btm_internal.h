@@ -116,7 +116,7 @@ struct GroupedCall {
 int configure_gemm_grouped_kernels();
 int configure_gemm_grouped_pair_kernels();
 int launch_gemm_grouped_pair(const GroupedCall &c, cudaStream_t st, int sm_count, const CUtensorMap &tmA, const CUtensorMap &tmA_band,
-                             const CUtensorMap &tmB, const CUtensorMap &tmC, GemmParams p);
+                             const CUtensorMap &tmB, const CUtensorMap &tmC, const GemmParams &p);
 int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int *status);
 long long grouped_slot_bound(int groups, int rows);
 // Microscaled 4-bit operands (mxfp4.cu). offsets == NULL: every group has rows / groups rows.

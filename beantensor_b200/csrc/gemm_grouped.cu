@@ -464,13 +464,15 @@ int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int
         rc = encode_tmap_3d(&tmC, c.dtype, c.C, (uint64_t)c.N, (uint64_t)p.M, (uint64_t)p.batch, pc, p.batch > 1 ? (uint64_t)c.strideC * 2 : pc, 64, 32);
         if (rc) return rc;
     }
-    // Pairs of CTAs when the groups are tall and deep enough. BTM_FORCE_KERNEL=1cta|2cta as for the dense products.
-    const long long pair_slots = c.wgrad ? (long long)c.groups * ((c.M + 255) / 256) : c.rows / 256;
-    bool pair = c.wgrad ? c.M > 128 && c.rows / c.groups >= 512 : c.rows / c.groups >= 512 && c.K >= 512;
-    pair = pair && pair_slots * ((c.N + 255) / 256) >= sm_count / 4;
+    // Pairs of CTAs for tall and deep groups. Measured, one CTA against pairs, bf16, rows / N x K:
+    //   16384 in 8 groups, 4096 x 4096: 482 / 429 us       16384 in 16, 2048 x 4096: 266 / 241      12000 in 4, 2560 x 2560: 126 / 118
+    //   8192 in 8, 1024 x 1024: 23.1 / 22.3                16384 in 64, 2048 x 2048: 158 / 172      4096 in 16, 1024 x 512: 11.6 / 13.3
+    // so from 512 rows per group and K = 1024 on, with half as many tiles as there are pairs. BTM_FORCE_KERNEL=1cta|2cta as
+    // for the dense products. The weight gradient has no pair form (gemm_grouped_pair.cu).
+    bool pair = !c.wgrad && c.rows / c.groups >= 512 && c.K >= 1024 && (long long)(c.rows / 256) * ((c.N + 255) / 256) >= sm_count / 4;
     if (const char *force = getenv("BTM_FORCE_KERNEL")) {
         if (!strcmp(force, "1cta")) pair = false;
-        else if (!strcmp(force, "2cta")) pair = true;
+        else if (!strcmp(force, "2cta")) pair = !c.wgrad;
     }
     if (pair) return launch_gemm_grouped_pair(c, st, sm_count, tmA, tmA_band, tmB, tmC, p);
     const int grid = (int)(most < sm_count ? most : sm_count);

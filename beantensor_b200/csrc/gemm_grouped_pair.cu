@@ -9,9 +9,8 @@
 // Rows of a group are cut into slots of 256; in a group's last slot the second CTA may own no row: it then loads none of
 // A and stores nothing.
 //
-// Weight gradient: the k-block that the group's end cuts gets a stage of its own. Each CTA's loads of it complete on a
-// barrier of that CTA, its MMA warp zeroes the foreign rows in its own shared memory and arrives on the leader's
-// full[s]; for this full[s] takes two arrivals, one of each CTA, on every stage.
+// Products only: the weight gradient was built and measured on pairs too and was level with the one-CTA kernel at best (16384
+// rows in 8 groups 505 against 504 us, in 64 groups 221 against 185 us), so it stays there.
 #include <cstring>
 
 #include <cuda_bf16.h>
@@ -65,15 +64,12 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                          const __grid_constant__ CUtensorMap tmC, const __grid_constant__ GemmParams p, const GroupedTables tab)
 {
     using namespace gp;
-    constexpr bool kWgrad = MODE == GROUPED_WGRAD;
     constexpr bool kBMnMajor = MODE != GROUPED_NK;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_full[STAGES];   // used in the leader
     __shared__ __align__(8) uint64_t bar_empty[STAGES];  // per CTA
     __shared__ __align__(8) uint64_t bar_tmem_full[2];   // per CTA
     __shared__ __align__(8) uint64_t bar_tmem_empty[2];  // used in the leader
-    __shared__ __align__(8) uint64_t bar_clean[STAGES];  // used in the leader: both CTAs have zeroed it
-    __shared__ __align__(8) uint64_t bar_cut[STAGES];    // per CTA: the cut k-block in this stage has landed (gradient)
     __shared__ uint32_t tmem_base_holder;
     __shared__ int abort_flag;
 
@@ -85,9 +81,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&bar_full[s]), 1);
-            mbar_init(smem_u32(&bar_clean[s]), 2);
             mbar_init(smem_u32(&bar_empty[s]), 1);
-            mbar_init(smem_u32(&bar_cut[s]), 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(smem_u32(&bar_tmem_full[a]), 1);
@@ -96,7 +90,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         fence_mbar_init();
         prefetch_tmap(&tmA);
         prefetch_tmap(&tmB);
-        if (!kWgrad) prefetch_tmap(&tmA_band);
+        prefetch_tmap(&tmA_band);
     }
     if (warp == 1) {
         tmem_alloc<2>(smem_u32(&tmem_base_holder), TMEM_COLS);
@@ -114,7 +108,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     walk.init(tab.offsets, tab.groups, tab.rows);
     const int group_slots = walk.count_slots();
     if (blockIdx.x == 0 && warp == 0) walk.report(p.status);
-    const GroupedPlan plan = plan_tiles<BN, 128>(kWgrad ? tab.groups * p.tiles_m : group_slots, p.N, num_pairs);
+    const GroupedPlan plan = plan_tiles<BN, 128>(group_slots, p.N, num_pairs);
 
     // Producer and issuer run as whole warps with uniform control flow; one elected lane issues (mbar_wait_uniform).
     if (warp == 0) {
@@ -123,20 +117,17 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         uint32_t phase = 0;
         bool ok = !p.debug_skip_loads;
         for (int tile = pair_id; ok && tile < plan.total; tile += num_pairs) {
-            const GroupedTile t = grouped_tile_uniform<kWgrad, PAIR_M>(p, plan, walk, tile);
-            const int k_rows = t.hi - t.lo; // gradient: the reduction
-            const int num_kb = kWgrad ? k_rows / BK : p.num_kb;
+            const GroupedTile t = grouped_tile_uniform<false, PAIR_M>(p, plan, walk, tile);
             const int half_bn = t.bn >> 1, chunks = half_bn >> 6;
             const int am = t.m0 + (int)rank * CTA_M, bn0 = t.n0 + (int)rank * half_bn;
-            // 32-row bands of A that belong to the group, of this CTA and of the pair (product)
-            const int pair_bands = kWgrad ? 8 : min(4, (t.hi - t.m0 + A_BAND - 1) / A_BAND) + min(4, max(0, t.hi - t.m0 - CTA_M + A_BAND - 1) / A_BAND);
-            const int bands = kWgrad ? 4 : min(4, max(0, t.hi - am + A_BAND - 1) / A_BAND);
+            // 32-row bands of A that belong to the group, of this CTA and of the pair
+            const int pair_bands = min(4, (t.hi - t.m0 + A_BAND - 1) / A_BAND) + min(4, max(0, t.hi - t.m0 - CTA_M + A_BAND - 1) / A_BAND);
+            const int bands = min(4, max(0, t.hi - am + A_BAND - 1) / A_BAND);
             const uint32_t kb_bytes = (uint32_t)(pair_bands * A_BAND * 128 + 2 * chunks * CHUNK_BYTES);
-            const int zb = kWgrad ? 0 : t.g;
-            for (int kb = 0; kb < num_kb; kb += KPS) {
+            for (int kb = 0; kb < p.num_kb; kb += KPS) {
                 ok = mbar_wait_uniform<true>(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
                 if (!ok) break;
-                const int nsub = min(KPS, num_kb - kb);
+                const int nsub = min(KPS, p.num_kb - kb);
                 if (elect_one()) {
                     const uint32_t full_local = smem_u32(&bar_full[stage]), full = map_to_leader(full_local);
                     if (rank == 0) mbar_expect_tx(full_local, kb_bytes * (uint32_t)nsub);
@@ -144,11 +135,8 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                     for (int sub = 0; sub < KPS; ++sub) {
                         if (sub < nsub) {
                             const uint32_t a0 = smem_base + stage * STAGE_BYTES + sub * KB_BYTES, b0 = a0 + A_BYTES;
-                            const int k0 = (kWgrad ? t.lo : 0) + (kb + sub) * BK;
-                            if constexpr (kWgrad) {
-                                tma_load_3d_2sm(a0, &tmA, am, k0, 0, full);
-                                tma_load_3d_2sm(a0 + CHUNK_BYTES, &tmA, am + 64, k0, 0, full);
-                            } else if (bands == 4) {
+                            const int k0 = (kb + sub) * BK;
+                            if (bands == 4) {
                                 tma_load_3d_2sm(a0, &tmA, k0, am, 0, full);
                             } else {
                                 for (int b = 0; b < bands; ++b) tma_load_3d_2sm(a0 + b * A_BAND * 128, &tmA_band, k0, am + b * A_BAND, 0, full);
@@ -156,8 +144,8 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
 #pragma unroll
                             for (int c = 0; c < BN / 128; ++c) {
                                 if (c < chunks) {
-                                    if (kBMnMajor) tma_load_3d_2sm(b0 + c * CHUNK_BYTES, &tmB, bn0 + c * 64, k0, zb, full);
-                                    else tma_load_3d_2sm(b0 + c * CHUNK_BYTES, &tmB, k0, bn0 + c * 64, zb, full);
+                                    if (kBMnMajor) tma_load_3d_2sm(b0 + c * CHUNK_BYTES, &tmB, bn0 + c * 64, k0, t.g, full);
+                                    else tma_load_3d_2sm(b0 + c * CHUNK_BYTES, &tmB, k0, bn0 + c * 64, t.g, full);
                                 }
                             }
                         }
@@ -169,101 +157,49 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
                     phase ^= 1u;
                 }
             }
-            if (kWgrad && ok && (k_rows & (BK - 1)) != 0) {
-                ok = mbar_wait_uniform<true>(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
-                if (ok) {
-                    if (elect_one()) {
-                        const uint32_t cut = smem_u32(&bar_cut[stage]), a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
-                        const int k0 = t.lo + num_kb * BK;
-                        mbar_expect_tx(cut, (uint32_t)(A_BYTES + chunks * CHUNK_BYTES));
-                        tma_load_3d(a0, &tmA, am, k0, 0, cut);
-                        tma_load_3d(a0 + CHUNK_BYTES, &tmA, am + 64, k0, 0, cut);
-                        for (int c = 0; c < chunks; ++c) tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, bn0 + c * 64, k0, 0, cut);
-                    }
-                    __syncwarp();
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                }
-            }
         }
-    } else if (warp == 1 && (rank == 0 || kWgrad)) {
-        // ------------------------------------------------------------ MMA issuer (leader), zeroing of cut k-blocks (both)
+    } else if (warp == 1 && rank == 0) {
+        // ------------------------------------------------------------ MMA issuer (leader)
         constexpr uint32_t kFmt = DT == BTM_BF16 ? 1u : 0u;
-        constexpr uint32_t a_step = (kWgrad ? 16 * 128 : 32) >> 4, b_step = (kBMnMajor ? 16 * 128 : 32) >> 4;
+        constexpr uint32_t a_step = 32 >> 4, b_step = (kBMnMajor ? 16 * 128 : 32) >> 4;
         const uint32_t tmem_u = uniform(tmem_base);
         int stage = 0, it = 0;
-        uint32_t full_phases = 0, cut_phases = 0; // one bit per stage
+        uint32_t phase = 0;
         bool ok = true;
         for (int tile = pair_id; ok && tile < plan.total; tile += num_pairs, ++it) {
-            const GroupedTile t = grouped_tile_uniform<kWgrad, PAIR_M>(p, plan, walk, tile);
-            const int k_rows = t.hi - t.lo;
-            const int num_kb = kWgrad ? k_rows / BK : p.num_kb;
-            const int left = kWgrad ? k_rows & (BK - 1) : 0; // rows of the cut k-block
-            const uint32_t idesc = make_idesc(kFmt, kWgrad, kBMnMajor, PAIR_M, (uint32_t)t.bn);
+            const GroupedTile t = grouped_tile_uniform<false, PAIR_M>(p, plan, walk, tile);
+            const uint32_t idesc = make_idesc(kFmt, false, kBMnMajor, PAIR_M, (uint32_t)t.bn);
             const int acc = it & 1;
             const uint32_t d_tmem = tmem_u + (uint32_t)(acc * BN);
-            if (rank == 0) {
-                ok = mbar_wait_uniform<true>(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
+            ok = mbar_wait_uniform<true>(smem_u32(&bar_tmem_empty[acc]), ((uint32_t)(it >> 1) & 1u) ^ 1u, &abort_flag, p.status, WAIT_MMA_TMEM_EMPTY, p.wait_limit);
+            tc_fence_after();
+            for (int kb = 0; ok && kb < p.num_kb; kb += KPS) {
+                ok = mbar_wait_uniform<true>(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
+                if (!ok) break;
                 tc_fence_after();
-                for (int kb = 0; ok && kb < num_kb; kb += KPS) {
-                    ok = mbar_wait_uniform<true>(smem_u32(&bar_full[stage]), (full_phases >> stage) & 1u, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const int nsub = min(KPS, num_kb - kb);
-                    const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
-                    const uint64_t ad = kWgrad ? make_smem_desc_sw128(a0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(a0, 16, 1024);
-                    const uint64_t bd = kBMnMajor ? make_smem_desc_sw128(b0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(b0, 16, 1024);
-                    if (elect_one()) {
+                const int nsub = min(KPS, p.num_kb - kb);
+                const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
+                const uint64_t ad = make_smem_desc_sw128(a0, 16, 1024);
+                const uint64_t bd = kBMnMajor ? make_smem_desc_sw128(b0, CHUNK_BYTES, 1024) : make_smem_desc_sw128(b0, 16, 1024);
+                if (elect_one()) {
 #pragma unroll
-                        for (int sub = 0; sub < KPS; ++sub) {
-                            if (sub < nsub) {
+                    for (int sub = 0; sub < KPS; ++sub) {
+                        if (sub < nsub) {
 #pragma unroll
-                                for (int ks = 0; ks < BK / 16; ++ks)
-                                    umma<2, false>(d_tmem, ad + (uint64_t)((sub * KB_BYTES >> 4) + ks * a_step), bd + (uint64_t)((sub * KB_BYTES >> 4) + ks * b_step),
-                                                   idesc, (uint32_t)((kb | sub | ks) != 0));
-                            }
+                            for (int ks = 0; ks < BK / 16; ++ks)
+                                umma<2, false>(d_tmem, ad + (uint64_t)((sub * KB_BYTES >> 4) + ks * a_step), bd + (uint64_t)((sub * KB_BYTES >> 4) + ks * b_step),
+                                               idesc, (uint32_t)((kb | sub | ks) != 0));
                         }
-                        umma_commit_2sm(smem_u32(&bar_empty[stage]), (uint16_t)3);
                     }
-                    __syncwarp();
-                    full_phases ^= 1u << stage;
-                    if (++stage == STAGES) stage = 0;
+                    umma_commit_2sm(smem_u32(&bar_empty[stage]), (uint16_t)3);
                 }
-            } else {
-                stage = (stage + (num_kb + KPS - 1) / KPS) % STAGES; // the whole k-blocks' stages are the leader's business
-            }
-            if (kWgrad && ok && left != 0) {
-                ok = mbar_wait_uniform(smem_u32(&bar_cut[stage]), (cut_phases >> stage) & 1u, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
-                if (ok) {
-                    const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
-                    const int steps = (left + 15) / 16, dirty = steps * 16 - left;
-                    for (int i = lane; i < dirty * 8; i += 32) {
-                        const uint32_t off = (uint32_t)(left + (i >> 3)) * 128u + (uint32_t)(i & 7) * 16u;
-                        for (int c = 0; c < CTA_M / 64; ++c) st_shared_v4(a0 + c * CHUNK_BYTES + off, 0u, 0u, 0u, 0u);
-                        for (int c = 0; c < t.bn / 128; ++c) st_shared_v4(b0 + c * CHUNK_BYTES + off, 0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(smem_u32(&bar_clean[stage]), 0);
-                    __syncwarp();
-                    if (rank == 0) {
-                        ok = mbar_wait_uniform<true>(smem_u32(&bar_clean[stage]), (cut_phases >> stage) & 1u, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
-                        tc_fence_after();
-                        if (ok && elect_one()) {
-                            const uint64_t ad = make_smem_desc_sw128(a0, CHUNK_BYTES, 1024), bd = make_smem_desc_sw128(b0, CHUNK_BYTES, 1024);
-                            for (int ks = 0; ks < steps; ++ks)
-                                umma<2, false>(d_tmem, ad + (uint64_t)(ks * a_step), bd + (uint64_t)(ks * b_step), idesc, (uint32_t)((num_kb | ks) != 0));
-                            umma_commit_2sm(smem_u32(&bar_empty[stage]), (uint16_t)3);
-                        }
-                        __syncwarp();
-                    }
-                    cut_phases ^= 1u << stage;
-                    if (++stage == STAGES) stage = 0;
+                __syncwarp();
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
-            if (rank == 0 && ok && elect_one()) umma_commit_2sm(smem_u32(&bar_tmem_full[acc]), (uint16_t)3);
+            if (ok && elect_one()) umma_commit_2sm(smem_u32(&bar_tmem_full[acc]), (uint16_t)3);
             __syncwarp();
         }
     } else if (warp >= 2) {
@@ -273,12 +209,12 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         uint32_t epi_tiles = 0;
         int it = 0;
         for (int tile = pair_id; tile < plan.total; tile += num_pairs, ++it) {
-            const GroupedTile t = grouped_tile<kWgrad, PAIR_M>(p, plan, walk, tile);
+            const GroupedTile t = grouped_tile<false, PAIR_M>(p, plan, walk, tile);
             const int acc = it & 1;
             if (!mbar_wait_warp<true>(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();
-            grouped_band<DT, kWgrad>(p, tmC, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t,
-                                     t.m0 + (int)rank * CTA_M + quad * 32, kWgrad ? p.M : t.hi, kWgrad && t.lo == t.hi, epi_smem, epi_tiles, lane);
+            grouped_band<DT, false>(p, tmC, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t,
+                                     t.m0 + (int)rank * CTA_M + quad * 32, t.hi, false, epi_smem, epi_tiles, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -349,13 +285,10 @@ static int launch_pair_mode(const GroupedCall &c, cudaStream_t st, int sm_count,
 }
 
 int launch_gemm_grouped_pair(const GroupedCall &c, cudaStream_t st, int sm_count, const CUtensorMap &tmA, const CUtensorMap &tmA_band,
-                             const CUtensorMap &tmB, const CUtensorMap &tmC, GemmParams p)
+                             const CUtensorMap &tmB, const CUtensorMap &tmC, const GemmParams &p)
 {
-    if (c.wgrad) p.tiles_m = (c.M + gp::PAIR_M - 1) / gp::PAIR_M;
-    p.group_m = 8;
 #define BTM_GROUPED_PAIR_CASE(DT)                                                                                             \
     do {                                                                                                                      \
-        if (c.wgrad) return launch_pair_mode<DT, GROUPED_WGRAD>(c, st, sm_count, tmA, tmA_band, tmB, tmC, p);                 \
         if (c.b_trans) return launch_pair_mode<DT, GROUPED_NK>(c, st, sm_count, tmA, tmA_band, tmB, tmC, p);                  \
         return launch_pair_mode<DT, GROUPED_KN>(c, st, sm_count, tmA, tmA_band, tmB, tmC, p);                                 \
     } while (0)
@@ -369,7 +302,6 @@ static cudaError_t raise_pair_smem()
 {
     cudaError_t e = cudaFuncSetAttribute(gemm_grouped_pair_kernel<DT, GROUPED_KN>, cudaFuncAttributeMaxDynamicSharedMemorySize, gp::SMEM_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(gemm_grouped_pair_kernel<DT, GROUPED_NK>, cudaFuncAttributeMaxDynamicSharedMemorySize, gp::SMEM_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(gemm_grouped_pair_kernel<DT, GROUPED_WGRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, gp::SMEM_BYTES);
     return e;
 }
 

@@ -112,24 +112,8 @@ __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensor
     if (row0 >= rows_end) return;
     const int z = kWgrad ? t.g : 0;
     const long long base = (long long)z * p.strideC;
-    if (!p.c_vec_ok) {
-        const int row = row0 + lane;
-#pragma unroll 1
-        for (int c = 0; c < t.bn / 32; ++c) {
-            uint32_t v[32];
-            tmem_ld_32x32(tmem_band + (uint32_t)(c * 32), v);
-            tmem_ld_wait();
-            if (zero) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = 0u;
-            }
-            const int col = t.n0 + c * 32, valid = min(32, p.N - col);
-            if (row < rows_end && valid > 0) store_row_direct<DT>(p, v, base + (long long)row * p.ldc + col, valid);
-        }
-        return;
-    }
     const uint32_t swz = (uint32_t)(lane & 7);
-    const bool whole = kWgrad || row0 + 32 <= rows_end; // C[g] is clipped by its tensor map
+    const bool whole = p.c_vec_ok && (kWgrad || row0 + 32 <= rows_end); // C[g] is clipped by its tensor map
 #pragma unroll 1
     for (int c = 0; c < t.bn / 64; ++c) {
         const int col = t.n0 + c * 64;
@@ -159,6 +143,24 @@ __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensor
                 tma_store_3d(&tmC, buf, col, row0, z);
                 bulk_commit();
             }
+        } else if (!p.c_vec_ok) {
+            // Rows of C that start anywhere: two bytes per lane, a warp writes 64 contiguous bytes of a row.
+            __syncwarp();
+            uint16_t *dst = reinterpret_cast<uint16_t *>(p.C[0]);
+            const int rows = min(32, rows_end - row0), cols = min(64, p.N - col);
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) {
+                const long long off = base + (long long)(row0 + r) * p.ldc + col;
+                if (!store_in_bounds(p, off, cols)) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int e = h * 32 + lane;
+                    uint16_t v;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(buf + (uint32_t)r * 128u + ((((uint32_t)(e >> 3)) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(e & 7) * 2u));
+                    if (e < cols) dst[off + e] = v;
+                }
+            }
+            if (lane == 0) bulk_commit();
         } else {
             __syncwarp();
             uint16_t *dst = reinterpret_cast<uint16_t *>(p.C[0]);
