@@ -39,9 +39,11 @@ constexpr int BN = 256;                 // widest tile
 constexpr int BK = 64;                  // k per stage: 128 bytes
 constexpr int CHUNK_BYTES = 64 * 128;   // every TMA box of an operand is 64 rows x 128 bytes, except A of the product
 constexpr int A_BYTES = BM * 128;
-constexpr int STAGE_BYTES = A_BYTES + BN * 128;
-constexpr int STAGES = 4;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_SMEM_BYTES + 1024;
+// The ring holds as many stages as fit at the launch's tile width: 4 at 256 columns, 6 at 128, 8 at 64, so that a launch
+// of narrow tiles (few rows: the time is the latency of the weights) asks for as many bytes ahead.
+constexpr int RING_BYTES = 4 * (A_BYTES + BN * 128);
+constexpr int STAGES = 8;
+constexpr int SMEM_BYTES = RING_BYTES + EPI_SMEM_BYTES + 1024;
 constexpr int TMEM_COLS = 512;
 constexpr int THREADS = 192;
 constexpr int A_BAND = 32;              // rows of a short A box: a tile with few rows does not fetch its neighbours'
@@ -97,6 +99,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (blockIdx.x == 0 && warp == 0) walk.report(p.status);
     const GroupedPlan plan = plan_tiles<gg::BN>(kWgrad ? tab.groups * p.tiles_m : group_slots, p.N, gridDim.x);
 
+    const uint32_t stage_bytes = (uint32_t)(A_BYTES + plan.bn * 128);
+    const int stages = min(STAGES, (int)((uint32_t)RING_BYTES / stage_bytes));
+
     // Producer and issuer run as whole warps with uniform control flow; one elected lane issues (mbar_wait_uniform).
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
@@ -115,7 +120,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 if (!ok) break;
                 if (elect_one()) {
                     const uint32_t full = smem_u32(&bar_full[stage]);
-                    const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
+                    const uint32_t a0 = smem_base + (uint32_t)stage * stage_bytes, b0 = a0 + A_BYTES;
                     const int k0 = kWgrad ? t.lo + kb * BK : kb * BK;
                     mbar_expect_tx(full, bytes);
                     if constexpr (kWgrad) {
@@ -135,7 +140,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     }
                 }
                 __syncwarp();
-                if (++stage == STAGES) {
+                if (++stage == stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
@@ -161,7 +166,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             for (int kb = 0; kb < num_kb; ++kb) {
                 ok = mbar_wait_uniform(smem_u32(&bar_full[stage]), phase, &abort_flag, p.status, WAIT_MMA_FULL, p.wait_limit);
                 if (!ok) break;
-                const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
+                const uint32_t a0 = smem_base + (uint32_t)stage * stage_bytes, b0 = a0 + A_BYTES;
                 int steps = BK / 16;
                 if (kWgrad) {
                     const int left = t.hi - t.lo - kb * BK; // rows of the group in this k-block
@@ -189,7 +194,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     umma_commit(smem_u32(&bar_empty[stage]));
                 }
                 __syncwarp();
-                if (++stage == STAGES) {
+                if (++stage == stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
@@ -200,7 +205,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     } else {
         // ------------------------------------------------------------ epilogue (warps 2..5)
         const int quad = warp & 3;
-        const uint32_t epi_smem = smem_base + STAGES * STAGE_BYTES + (uint32_t)quad * EPI_WARP_BYTES;
+        const uint32_t epi_smem = smem_base + RING_BYTES + (uint32_t)quad * EPI_WARP_BYTES;
         uint32_t epi_tiles = 0;
         int it = 0;
         for (int tile = blockIdx.x; tile < plan.total; tile += gridDim.x, ++it) {

@@ -44,6 +44,7 @@ __device__ __forceinline__ GroupedPlan plan_tiles(int slots, int N, int ctas)
         }
     }
     best.total = uniform(best.total);
+    best.bn = uniform(best.bn);
     return best;
 }
 
