@@ -163,14 +163,33 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
 
 // The wait for a warp that then issues tcgen05 or TMA instructions: all lanes poll and vote, so that control flow stays
 // uniform in the compiler's eyes and what the issue needs (descriptors, coordinates) can live in uniform registers. Moved there
-// one by one from a single-lane branch they cost the issuing warp about 100 cycles per tcgen05.mma instead of 36.
+// one by one from a single-lane branch they cost the issuing warp about 100 cycles per tcgen05.mma instead of 36. Polls
+// are short: these waits are the hand-offs of the ring, and a sleeping warp takes hundreds of cycles to wake.
+template <bool kCluster = false>
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    if constexpr (kCluster)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    else
+        return mbar_try_wait_short(bar, parity);
+    return ok != 0;
+}
 template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait_uniform(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code, long long limit_cycles)
 {
-    if (__all_sync(0xffffffffu, kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) return true;
+    if (__all_sync(0xffffffffu, mbar_poll<kCluster>(bar, parity))) return true;
     const long long t0 = clock64();
+    int turns = 0;
     while (true) {
-        if (__all_sync(0xffffffffu, kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) return true;
+        if (__all_sync(0xffffffffu, mbar_poll<kCluster>(bar, parity))) return true;
+        if ((++turns & 63) != 0) continue; // the clock and the abort flag only now and then
         const bool late = clock64() - t0 > limit_cycles;
         if (__any_sync(0xffffffffu, late || *abort_flag != 0)) {
             if ((threadIdx.x & 31) == 0 && *abort_flag == 0) {

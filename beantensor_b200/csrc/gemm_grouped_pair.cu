@@ -211,7 +211,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         for (int tile = pair_id; tile < plan.total; tile += num_pairs, ++it) {
             const GroupedTile t = grouped_tile<false, PAIR_M>(p, plan, walk, tile);
             const int acc = it & 1;
-            if (!mbar_wait_warp<true>(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
+            if (!mbar_wait_uniform<true>(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();
             grouped_band<DT, false>(p, tmC, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t,
                                      t.m0 + (int)rank * CTA_M + quad * 32, t.hi, false, epi_smem, epi_tiles, lane);

@@ -22,27 +22,32 @@ struct GroupedPlan {
 
 // Cost of a tile in units of B columns: its columns plus kTileOverhead for what does not shrink with the width (the A
 // rows, the hand-offs). Waves are counted whole, a last one that fits twice over is run as half-width tiles.
+template <int kWidth, int kNarrowest>
+__device__ __forceinline__ void try_width(GroupedPlan &best, long long &best_cost, int slots, int N, int ctas)
+{
+    constexpr int kTileOverhead = 64;
+    const unsigned tiles_n = (unsigned)(N + kWidth - 1) / kWidth;
+    const unsigned tiles = (unsigned)slots * tiles_n;
+    const unsigned waves = tiles / (unsigned)ctas, rem = tiles - waves * (unsigned)ctas;
+    const bool halves = kWidth % 128 == 0 && kWidth / 2 >= kNarrowest && rem > 0 && 2 * rem <= (unsigned)ctas;
+    const long long cost = (long long)waves * (kWidth + kTileOverhead) + (rem == 0 ? 0 : (halves ? kWidth / 2 : kWidth) + kTileOverhead);
+    if (cost < best_cost) {
+        best_cost = cost;
+        best.bn = kWidth;
+        best.tiles_n = (int)tiles_n;
+        best.full = (int)(halves ? tiles - rem : tiles);
+        best.total = (int)(halves ? tiles + rem : tiles);
+    }
+}
+// Widths kWidest, 128 and 64, none below kNarrowest.
 template <int kWidest, int kNarrowest = 64>
 __device__ __forceinline__ GroupedPlan plan_tiles(int slots, int N, int ctas)
 {
-    constexpr int kTileOverhead = 64;
     GroupedPlan best;
     long long best_cost = 0x7FFFFFFFFFFFFFFFLL;
-#pragma unroll
-    for (int bn = kWidest; bn >= kNarrowest; bn = bn > 128 ? 128 : bn / 2) {
-        const int tiles_n = (N + bn - 1) / bn;
-        const int tiles = slots * tiles_n;
-        const int waves = tiles / ctas, rem = tiles - waves * ctas;
-        const bool halves = bn % 128 == 0 && bn / 2 >= kNarrowest && rem > 0 && 2 * rem <= ctas;
-        const long long cost = (long long)waves * (bn + kTileOverhead) + (rem == 0 ? 0 : (halves ? bn / 2 : bn) + kTileOverhead);
-        if (cost < best_cost) {
-            best_cost = cost;
-            best.bn = bn;
-            best.tiles_n = tiles_n;
-            best.full = halves ? tiles - rem : tiles;
-            best.total = halves ? tiles + rem : tiles;
-        }
-    }
+    try_width<kWidest, kNarrowest>(best, best_cost, slots, N, ctas);
+    if (kWidest > 128) try_width<128, kNarrowest>(best, best_cost, slots, N, ctas);
+    if (kNarrowest < 128) try_width<64, kNarrowest>(best, best_cost, slots, N, ctas);
     best.total = uniform(best.total);
     best.bn = uniform(best.bn);
     return best;
@@ -65,10 +70,10 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const G
         tile = pl.full + (s >> 1);
         half = s & 1;
     }
-    const int slot = tile / pl.tiles_n;
+    const int slot = (int)((unsigned)tile / (unsigned)pl.tiles_n);
     int first, count; // the group's slots
     if (kWgrad) {
-        o.g = slot / p.tiles_m;
+        o.g = (int)((unsigned)slot / (unsigned)p.tiles_m);
         first = o.g * p.tiles_m;
         count = p.tiles_m;
         walk.find_group(o.g, o.lo, o.hi);
@@ -78,15 +83,19 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const G
     }
     // Within a group: bands of group_m row tiles, row tiles innermost, so that neighbouring CTAs share columns of B.
     const int r0 = tile - first * pl.tiles_n;
-    const int per_band = p.group_m * pl.tiles_n;
-    const int band = r0 / per_band;
-    const int first_m = band * p.group_m;
-    const int height = min(count - first_m, p.group_m);
-    const int r = r0 - band * per_band;
-    o.slot = first + first_m + r % height;
-    o.m0 = (kWgrad ? 0 : o.lo) + (first_m + r % height) * kSlot;
+    int first_m = 0, height = count, r = r0;
+    if (count > p.group_m) {
+        const int per_band = p.group_m * pl.tiles_n;
+        const int band = (int)((unsigned)r0 / (unsigned)per_band);
+        first_m = band * p.group_m;
+        height = min(count - first_m, p.group_m);
+        r = r0 - band * per_band;
+    }
+    const int rn = height == 1 ? r : (int)((unsigned)r / (unsigned)height), rm = r - rn * height;
+    o.slot = first + first_m + rm;
+    o.m0 = (kWgrad ? 0 : o.lo) + (first_m + rm) * kSlot;
     o.bn = half < 0 ? pl.bn : pl.bn / 2;
-    o.n0 = (r / height) * pl.bn + (half > 0 ? pl.bn / 2 : 0);
+    o.n0 = rn * pl.bn + (half > 0 ? pl.bn / 2 : 0);
     return o;
 }
 
@@ -121,14 +130,16 @@ __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensor
         if (col >= p.N) break;
         const uint32_t buf = epi_smem + (tile_count & 1u) * EPI_TILE_BYTES;
         ++tile_count;
-        if (lane == 0) bulk_wait_read<1>();
+        uint32_t v0[32], v1[32];
+        tmem_ld_32x32(tmem_band + (uint32_t)(c * 64), v0);
+        tmem_ld_32x32(tmem_band + (uint32_t)(c * 64 + 32), v1);
+        if (lane == 0) bulk_wait_read<1>(); // the store of two chunks ago has read this buffer
         __syncwarp();
+        tmem_ld_wait();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint32_t v[32], q[16];
-            tmem_ld_32x32(tmem_band + (uint32_t)(c * 64 + h * 32), v);
-            tmem_ld_wait();
-            pack16<DT>(v, q);
+            uint32_t q[16];
+            pack16<DT>(h == 0 ? v0 : v1, q);
             if (zero) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) q[j] = 0u;

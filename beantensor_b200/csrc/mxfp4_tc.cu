@@ -188,7 +188,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         for (int tile = blockIdx.x; tile < plan.total; tile += gridDim.x, ++it) {
             const GroupedTile t = grouped_tile<false, GROUP_SLOT_ROWS>(p, plan, walk, tile);
             const int acc = it & 1;
-            if (!mbar_wait_warp(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
+            if (!mbar_wait_uniform(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();
             grouped_band<DT, false>(p, tmC, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t, t.m0 + quad * 32, t.hi, false,
                                     epi_smem, epi_tiles, lane);
