@@ -130,6 +130,7 @@ DeviceState *device_state(int device)
     if (configure_gemm_grouped_kernels()) return nullptr;
     if (configure_gemm_grouped_pair_kernels()) return nullptr;
     if (configure_mxfp4_kernels()) return nullptr;
+    if (configure_mxfp4_pair_kernels()) return nullptr;
     if (configure_int4_gemv_kernels()) return nullptr;
     ds->sm_count = prop.multiProcessorCount;
     ds->ready.store(true, std::memory_order_release);
@@ -142,6 +143,7 @@ int encode_tmap_3d(CUtensorMap *out, int dtype, const void *base, uint64_t d0, u
     CUtensorMapDataType dt = dtype == BTM_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                              : dtype == BTM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                              : dtype == BTM_U8   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                             : dtype == BTM_U32  ? CU_TENSOR_MAP_DATA_TYPE_UINT32
                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     cuuint64_t dims[3] = {d0, d1, d2};
     cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};

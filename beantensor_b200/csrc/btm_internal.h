@@ -134,6 +134,9 @@ struct Mxfp4Call {
     long long ldo;
 };
 int configure_mxfp4_kernels();
+int configure_mxfp4_pair_kernels();
+int launch_mxfp4_matmul_pair(const Mxfp4Call &c, cudaStream_t st, int sm_count, const GemmParams &p, const CUtensorMap &tmA, const CUtensorMap &tmA_band,
+                             const CUtensorMap &tmC);
 int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *status);
 // Fills `cm` for the destinations in `p` (no-op when p.c_vec_ok == 0: the general store path needs no maps).
 int encode_store_maps(StoreMaps *cm, int dtype, const GemmParams &p);

@@ -168,8 +168,10 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
 template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity)
 {
-    uint32_t ok;
-    if constexpr (kCluster)
+    if constexpr (!kCluster) {
+        return mbar_try_wait_short(bar, parity);
+    } else {
+        uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
@@ -177,9 +179,8 @@ __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity)
             : "=r"(ok)
             : "r"(bar), "r"(parity)
             : "memory");
-    else
-        return mbar_try_wait_short(bar, parity);
-    return ok != 0;
+        return ok != 0;
+    }
 }
 template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait_uniform(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code, long long limit_cycles)
@@ -232,6 +233,24 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
                  "r"(bar)
                  : "memory");
+}
+
+// ---------------------------------------------------------------- CTA pairs
+__device__ __forceinline__ uint32_t pair_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void pair_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_to_leader(uint32_t smem_addr)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr));
+    return r;
 }
 
 // ---------------------------------------------------------------- tcgen05 / tensor memory

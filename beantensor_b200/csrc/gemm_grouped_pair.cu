@@ -39,25 +39,6 @@ constexpr int THREADS = 192;
 constexpr int A_BAND = 32;
 } // namespace gp
 
-namespace {
-__device__ __forceinline__ uint32_t pair_rank()
-{
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void pair_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t map_to_leader(uint32_t smem_addr)
-{
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr));
-    return r;
-}
-} // namespace
-
 template <int DT, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(gp::THREADS, 1)
 gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA_band, const __grid_constant__ CUtensorMap tmB,

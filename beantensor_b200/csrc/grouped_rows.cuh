@@ -23,10 +23,13 @@ struct GroupWalk {
     // The window: groups g0 .. g0 + 31, lane l holding group g0 + l.
     int g0, floor_row, slots_before; // rows and slots in front of the window
     int lo, hi, incl;                // this lane's rows and the inclusive count of slots within the window
+    // For pairs also in single slots of GROUP_SLOT_ROWS, which is how the scales of a microscaled operand are counted.
+    int singles_before, incl_singles;
     int bad;
 
-    __device__ __forceinline__ void load(int first, int floor_at, int slots)
+    __device__ __forceinline__ void load(int first, int floor_at, int slots, int singles)
     {
+        singles_before = singles;
         g0 = first;
         floor_row = floor_at;
         slots_before = slots;
@@ -47,14 +50,28 @@ struct GroupWalk {
             const int o = __shfl_up_sync(0xffffffffu, incl, d);
             if (lane >= d) incl += o;
         }
+        if (kSlot == GROUP_SLOT_ROWS) {
+            incl_singles = incl;
+        } else {
+            incl_singles = (hi - lo + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, incl_singles, d);
+                if (lane >= d) incl_singles += o;
+            }
+        }
     }
-    __device__ __forceinline__ void next() { load(g0 + 32, __shfl_sync(0xffffffffu, hi, 31), slots_before + __shfl_sync(0xffffffffu, incl, 31)); }
+    __device__ __forceinline__ void next()
+    {
+        load(g0 + 32, __shfl_sync(0xffffffffu, hi, 31), slots_before + __shfl_sync(0xffffffffu, incl, 31),
+             singles_before + __shfl_sync(0xffffffffu, incl_singles, 31));
+    }
 
     __device__ __forceinline__ void first_window()
     {
         const int raw = offsets ? offsets[0] : 0, at = min(max(raw, 0), rows);
         bad |= raw != at ? 1 : 0;
-        load(0, at, 0);
+        load(0, at, 0, 0);
     }
     __device__ __forceinline__ void init(const int *offs, int n_groups, int n_rows)
     {
@@ -83,6 +100,11 @@ struct GroupWalk {
         row_lo = __shfl_sync(0xffffffffu, lo, l);
         row_hi = __shfl_sync(0xffffffffu, hi, l);
         first_slot = slots_before + __shfl_sync(0xffffffffu, incl, l) - (row_hi - row_lo + kSlot - 1) / kSlot;
+    }
+    // Single slots of the groups in front of `group`, which the last find_slot returned.
+    __device__ __forceinline__ int singles_of(int group, int rows_of_group) const
+    {
+        return singles_before + __shfl_sync(0xffffffffu, incl_singles, group - g0) - (rows_of_group + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS;
     }
     // The rows of `group`, which must not be below that of an earlier call.
     __device__ __forceinline__ void find_group(int group, int &row_lo, int &row_hi)

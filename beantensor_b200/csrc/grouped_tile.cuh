@@ -92,7 +92,9 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GemmParams &p, const G
         r = r0 - band * per_band;
     }
     const int rn = height == 1 ? r : (int)((unsigned)r / (unsigned)height), rm = r - rn * height;
-    o.slot = first + first_m + rm;
+    // slot: of GROUP_SLOT_ROWS rows, for a pair that of its first CTA
+    if (!kWgrad && kSlot != GROUP_SLOT_ROWS) o.slot = walk.singles_of(o.g, o.hi - o.lo) + (first_m + rm) * (kSlot / GROUP_SLOT_ROWS);
+    else o.slot = first + first_m + rm;
     o.m0 = (kWgrad ? 0 : o.lo) + (first_m + rm) * kSlot;
     o.bn = half < 0 ? pl.bn : pl.bn / 2;
     o.n0 = rn * pl.bn + (half > 0 ? pl.bn / 2 : 0);

@@ -7,6 +7,7 @@
 // tensor memory by one tcgen05.cp.
 // One persistent CTA per SM, warp roles and tile walk as in gemm_grouped.cu (a plain product is one group that owns every
 // row).
+#include <cstdlib>
 #include <cstring>
 
 #include <cuda_bf16.h>
@@ -258,6 +259,15 @@ int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
         rc = encode_tmap_3d(&tmC, c.dtype, c.out, (uint64_t)c.N, (uint64_t)c.rows, 1, (uint64_t)c.ldo * 2, (uint64_t)c.ldo * 2, 64, 32);
         if (rc) return rc;
     }
+    // Pairs of CTAs for tall groups and a reduction that pays for their set-up. Measured, one CTA against pairs, rows / N x K:
+    //   8192 / 11008 x 4096: 193 / 154 us    4096 / 4096 x 4096: 46.1 / 36.6    256 / 11008 x 4096: 11.9 / 10.4
+    //   16384 in 64 groups / 2048 x 2048: 63.2 / 60.5    8192 / 2048 x 1024: 17.2 / 17.9    3001 in 24 / 1000 x 1440: 15.9 / 17.4
+    bool pair = c.rows / c.groups >= 256 && c.K >= 1536;
+    if (const char *force = getenv("BTM_FORCE_KERNEL")) {
+        if (!strcmp(force, "1cta")) pair = false;
+        else if (!strcmp(force, "2cta")) pair = true;
+    }
+    if (pair) return launch_mxfp4_matmul_pair(c, st, sm_count, p, tmA, tmA_band, tmC);
     const MxOperands op = {(const uint8_t *)c.act_scales, (const uint8_t *)c.w_scales, c.offsets, c.groups, c.rows};
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));

@@ -22,6 +22,12 @@ def table(bounds):
     return torch.tensor(bounds, dtype=torch.int32, device="cuda")
 
 
+@pytest.fixture(params=["1cta", "2cta"])
+def kernel(request, monkeypatch):
+    """Both forms of the tensor-core product on every shape."""
+    monkeypatch.setenv("BTM_FORCE_KERNEL", request.param)
+
+
 def quantized(btm, x, offsets=None, groups=1):
     rows, K = x.shape
     packed = torch.full((rows, K // 2), 0xA5, dtype=torch.uint8, device="cuda")
@@ -152,7 +158,7 @@ SHAPES = [(1, 8, 32), (1, 136, 256), (2, 64, 64), (7, 200, 96), (16, 128, 128), 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("M,N,K", SHAPES)
-def test_product(btm, M, N, K, dtype):
+def test_product(btm, kernel, M, N, K, dtype):
     x, w = normal((M, K), BF16, 1), normal((N, K), BF16, 2, K ** -0.5)
     xq, xs = quantized(btm, x)
     wq, ws = quantized(btm, w)
@@ -164,7 +170,7 @@ def test_product(btm, M, N, K, dtype):
 
 
 @pytest.mark.parametrize("M,N,K,pad", [(40, 100, 128, 3), (130, 264, 320, 8), (1, 264, 320, 1), (200, 128, 64, 24)])
-def test_product_into_a_wider_output(btm, M, N, K, pad):
+def test_product_into_a_wider_output(btm, kernel, M, N, K, pad):
     x, w = normal((M, K), BF16, 1), normal((N, K), BF16, 2)
     wide = normal((M, N + 2 * pad), F16, 3)
     before = wide.clone()
@@ -175,7 +181,7 @@ def test_product_into_a_wider_output(btm, M, N, K, pad):
     assert torch.equal(wide[:, :pad], before[:, :pad]) and torch.equal(wide[:, pad + N:], before[:, pad + N:])
 
 
-def test_nan_blocks_spoil_their_row_and_column_only(btm):
+def test_nan_blocks_spoil_their_row_and_column_only(btm, kernel):
     M, N, K = 150, 140, 288
     x, w = normal((M, K), F32, 1), normal((N, K), F32, 2)
     x[3, 200], w[137, 287] = float("nan"), float("inf")
@@ -189,7 +195,7 @@ def test_nan_blocks_spoil_their_row_and_column_only(btm):
     ragged.check(torch.where(bad, 0, out), torch.where(bad, 0.0, exact), mass, K)
 
 
-def test_extreme_scales(btm):
+def test_extreme_scales(btm, kernel):
     # 2^-127 and 2^125 in one product: the factors meet exactly, nothing is flushed in between.
     M, N, K = 20, 24, 64
     x, w = torch.zeros((M, K), device="cuda"), torch.zeros((N, K), device="cuda")
@@ -204,7 +210,7 @@ def test_extreme_scales(btm):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("N,K", [(8, 32), (136, 256), (1001, 416), (264, 1440), (640, 96)])
 @pytest.mark.parametrize("bounds", BOUNDS + [[0, 0, 1, 1, 1, 2], [0, 1], [0, 700, 701, 1500]])
-def test_grouped_product(btm, bounds, N, K, dtype):
+def test_grouped_product(btm, kernel, bounds, N, K, dtype):
     rows, groups = bounds[-1] + 11, len(bounds) - 1
     x = normal((rows, K), BF16, 1)
     w = normal((groups * N, K), BF16, 2, K ** -0.5).reshape(groups, N, K)
@@ -226,7 +232,7 @@ def test_grouped_product(btm, bounds, N, K, dtype):
         assert torch.equal(out[part].view(torch.int16), before[part].view(torch.int16))
 
 
-def test_empty_calls(btm):
+def test_empty_calls(btm, kernel):
     by = lambda *s: torch.empty(s, dtype=torch.uint8, device="cuda")  # noqa: E731
     wq, ws = quantized(btm, normal((40, 64), BF16, 1))
     btm.quantize_mxfp4_gpu(torch.empty((0, 64), dtype=F16, device="cuda"), by(0, 32), by(0))
@@ -239,7 +245,7 @@ def test_empty_calls(btm):
     assert (out == 0).all()
 
 
-def test_captured_experts_with_another_table(btm):
+def test_captured_experts_with_another_table(btm, kernel):
     rows, groups, N, K = 200, 6, 264, 192
     x, w = normal((rows, K), BF16, 1), normal((groups * N, K), BF16, 2).reshape(groups, N, K)
     wq = torch.empty((groups, N, K // 2), dtype=torch.uint8, device="cuda")
@@ -266,7 +272,7 @@ def test_captured_experts_with_another_table(btm):
         assert (out[bounds[-1]:] == 0).all()
 
 
-def test_two_layers_in_4_bits(btm):
+def test_two_layers_in_4_bits(btm, kernel):
     # quantise -> product -> quantise -> product, back to back, every launch fed by the one before; twenty times the same bits
     M, K, H = 33, 512, 1056
     x, w1, w2 = normal((M, K), BF16, 1), normal((H, K), BF16, 2, K ** -0.5), normal((K, H), BF16, 3, H ** -0.5)
@@ -286,7 +292,7 @@ def test_two_layers_in_4_bits(btm):
         assert torch.equal(h, first[0]) and torch.equal(y, first[1])
 
 
-def test_experts_quantised_and_dense_agree(btm):
+def test_experts_quantised_and_dense_agree(btm, kernel):
     # The 4-bit product of experts against the 16-bit grouped product of the same values: both sum the same exact products.
     bounds, rows, groups, N, K = [0, 50, 50, 181, 200], 200, 4, 136, 256
     x, w = normal((rows, K), BF16, 1, 0.1), normal((groups * N, K), BF16, 2, 0.1).reshape(groups, N, K)
