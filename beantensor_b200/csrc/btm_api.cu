@@ -131,6 +131,7 @@ DeviceState *device_state(int device)
     if (configure_gemm_grouped_pair_kernels()) return nullptr;
     if (configure_mxfp4_kernels()) return nullptr;
     if (configure_mxfp4_pair_kernels()) return nullptr;
+    if (configure_grouped_decode_kernels()) return nullptr;
     if (configure_int4_gemv_kernels()) return nullptr;
     ds->sm_count = prop.multiProcessorCount;
     ds->ready.store(true, std::memory_order_release);

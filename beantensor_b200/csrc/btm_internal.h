@@ -115,6 +115,9 @@ struct GroupedCall {
 };
 int configure_gemm_grouped_kernels();
 int configure_gemm_grouped_pair_kernels();
+int configure_grouped_decode_kernels();
+bool grouped_decode_fits(int groups, int rows, int N, int sm_count);
+int launch_grouped_decode(const GroupedCall &c, cudaStream_t st, int sm_count, int *status);
 int launch_gemm_grouped_pair(const GroupedCall &c, cudaStream_t st, int sm_count, const CUtensorMap &tmA, const CUtensorMap &tmA_band,
                              const CUtensorMap &tmB, const CUtensorMap &tmC, const GemmParams &p);
 int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int *status);
@@ -135,6 +138,7 @@ struct Mxfp4Call {
 };
 int configure_mxfp4_kernels();
 int configure_mxfp4_pair_kernels();
+int launch_mxfp4_decode(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *status);
 int launch_mxfp4_matmul_pair(const Mxfp4Call &c, cudaStream_t st, int sm_count, const GemmParams &p, const CUtensorMap &tmA, const CUtensorMap &tmA_band,
                              const CUtensorMap &tmC);
 int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *status);

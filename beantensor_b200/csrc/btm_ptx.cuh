@@ -227,6 +227,11 @@ __device__ __forceinline__ void tma_load_3d_2sm(uint32_t dst, const CUtensorMap 
         : "memory");
 }
 
+// Asks for a box to be brought into L2. A hint: nothing waits for it and no data is read.
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap *m, int x, int y, int z)
+{
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(m), "r"(x), "r"(y), "r"(z) : "memory");
+}
 // Untiled bulk copy global -> this CTA's shared memory; addresses and size are multiples of 16 bytes.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
 {

@@ -429,6 +429,10 @@ int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int
     const bool tc = mult16(c.A, c.lda) && mult16(c.B, c.ldb) && (c.wgrad || c.groups == 1 || (c.strideB * 2) % 16 == 0) && c.rows > 0 &&
                     (c.wgrad || c.K > 0);
     if (!tc) return launch_grouped_simt(c, st, status);
+    const char *force = getenv("BTM_FORCE_KERNEL"); // 1cta, 2cta or decode: the tests run every shape on each
+    bool decode = !c.wgrad && grouped_decode_fits(c.groups, c.rows, c.N, sm_count);
+    if (force) decode = !c.wgrad && !strcmp(force, "decode");
+    if (decode) return launch_grouped_decode(c, st, sm_count, status);
     const long long bound = c.wgrad ? (long long)c.groups * ((c.M + BM - 1) / BM) : grouped_slot_bound(c.groups, c.rows);
     const long long most = bound * ((c.N + 63) / 64); // tiles at the smallest width
     if (most > 0x3FFFFFFFLL) return set_error(BTM_ERR_UNSUPPORTED, "grouped matmul: too many output tiles (%lld)", most);
@@ -472,10 +476,9 @@ int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int
     // Pairs of CTAs for tall and deep groups. Measured, one CTA against pairs, bf16, rows / N x K:
     //   16384 in 8 groups, 4096 x 4096: 482 / 429 us       16384 in 16, 2048 x 4096: 266 / 241      12000 in 4, 2560 x 2560: 126 / 118
     //   8192 in 8, 1024 x 1024: 23.1 / 22.3                16384 in 64, 2048 x 2048: 158 / 172      4096 in 16, 1024 x 512: 11.6 / 13.3
-    // so from 512 rows per group and K = 1024 on, with half as many tiles as there are pairs. BTM_FORCE_KERNEL=1cta|2cta as
-    // for the dense products. The weight gradient has no pair form (gemm_grouped_pair.cu).
+    // so from 512 rows per group and K = 1024 on, with half as many tiles as there are pairs. The weight gradient has no pair form (gemm_grouped_pair.cu).
     bool pair = !c.wgrad && c.rows / c.groups >= 512 && c.K >= 1024 && (long long)(c.rows / 256) * ((c.N + 255) / 256) >= sm_count / 4;
-    if (const char *force = getenv("BTM_FORCE_KERNEL")) {
+    if (force) {
         if (!strcmp(force, "1cta")) pair = false;
         else if (!strcmp(force, "2cta")) pair = !c.wgrad;
     }

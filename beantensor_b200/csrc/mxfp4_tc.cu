@@ -231,6 +231,10 @@ int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
         z.dtype = c.dtype; z.groups = c.groups; z.rows = c.rows; z.N = c.N; z.offsets = c.offsets; z.C = c.out; z.ldc = c.ldo;
         return launch_gemm_grouped(z, st, sm_count, status);
     }
+    const char *force = getenv("BTM_FORCE_KERNEL"); // 1cta, 2cta or decode: the tests run every shape on each
+    bool decode = grouped_decode_fits(c.groups, c.rows, c.N, sm_count);
+    if (force) decode = !strcmp(force, "decode");
+    if (decode) return launch_mxfp4_decode(c, st, sm_count, status);
     const long long slots = grouped_slot_bound(c.groups, c.rows);
     const long long most = slots * ((c.N + 63) / 64);
     if (most > 0x3FFFFFFFLL) return set_error(BTM_ERR_UNSUPPORTED, "mxfp4 matmul: too many output tiles (%lld)", most);
@@ -263,7 +267,7 @@ int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
     //   8192 / 11008 x 4096: 193 / 154 us    4096 / 4096 x 4096: 46.1 / 36.6    256 / 11008 x 4096: 11.9 / 10.4
     //   16384 in 64 groups / 2048 x 2048: 63.2 / 60.5    8192 / 2048 x 1024: 17.2 / 17.9    3001 in 24 / 1000 x 1440: 15.9 / 17.4
     bool pair = c.rows / c.groups >= 256 && c.K >= 1536;
-    if (const char *force = getenv("BTM_FORCE_KERNEL")) {
+    if (force) {
         if (!strcmp(force, "1cta")) pair = false;
         else if (!strcmp(force, "2cta")) pair = true;
     }

@@ -33,9 +33,9 @@ def table(bounds):
     return torch.tensor(bounds, dtype=torch.int32, device="cuda")
 
 
-@pytest.fixture(params=["1cta", "2cta"])
+@pytest.fixture(params=["1cta", "2cta", "decode"])
 def kernel(request, monkeypatch):
-    """Both tensor-core kernels on every shape; operands that they cannot address take the general one either way."""
+    """Every tensor-core kernel on every shape; operands that they cannot address take the general one either way."""
     monkeypatch.setenv("BTM_FORCE_KERNEL", request.param)
 
 

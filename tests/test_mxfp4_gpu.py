@@ -22,9 +22,9 @@ def table(bounds):
     return torch.tensor(bounds, dtype=torch.int32, device="cuda")
 
 
-@pytest.fixture(params=["1cta", "2cta"])
+@pytest.fixture(params=["1cta", "2cta", "decode"])
 def kernel(request, monkeypatch):
-    """Both forms of the tensor-core product on every shape."""
+    """Every form of the tensor-core product on every shape."""
     monkeypatch.setenv("BTM_FORCE_KERNEL", request.param)
 
 
