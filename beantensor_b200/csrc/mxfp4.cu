@@ -5,6 +5,7 @@
 // is exact, so the only rounding is the one to four bits. A block that holds an infinity or a NaN has no such scale: it
 // gets scale 255 (NaN) and zero codes, and everything that it enters becomes NaN. Dequantise: q 2^X, rounded once.
 #include <cstring>
+#include <cstdlib>
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -18,8 +19,8 @@
 namespace btm {
 
 namespace mxq {
-constexpr int THREADS = 256; // 16 threads x 8 values across a scale block's 128 k, 16 rows at a time
-constexpr int ROWS = 16;
+constexpr int THREADS = 256;
+constexpr int ROWS = 16; // 16 threads x 8 values across a scale block's 128 k, 16 rows at a time
 constexpr int PASSES = GROUP_SLOT_ROWS / ROWS;
 } // namespace mxq
 
@@ -92,107 +93,151 @@ __device__ __forceinline__ SlotRows slot_rows(int slot, const int *offsets, int 
     return found;
 }
 
-// Eight consecutive values as they lie: 16 bytes of a 16-bit type, 32 of fp32.
+// One block of 32 consecutive values as they lie, as 32-bit words.
 template <typename T>
-struct Raw8 {
-    uint4 q[sizeof(T) / 2];
+struct RawBlock {
+    static constexpr int WORDS = MX_BLOCK * sizeof(T) / 4;
+    uint32_t w[WORDS];
 };
 
+// vec: 2 = 32-byte loads (the widest there are), 1 = 16-byte, 0 = element by element.
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8(const T *p, bool vec)
+__device__ __forceinline__ void load_block(RawBlock<T> &r, const T *p, int vec)
 {
-    Raw8<T> r;
-    if (vec) {
+    constexpr int W = RawBlock<T>::WORDS;
+    if (vec == 2) {
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.q[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+        for (int i = 0; i < W; i += 8)
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3]), "=r"(r.w[i + 4]), "=r"(r.w[i + 5]), "=r"(r.w[i + 6]),
+                           "=r"(r.w[i + 7])
+                         : "l"(reinterpret_cast<const uint32_t *>(p) + i));
+    } else if (vec == 1) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i);
+            r.w[i] = q.x; r.w[i + 1] = q.y; r.w[i + 2] = q.z; r.w[i + 3] = q.w;
+        }
     } else if constexpr (sizeof(T) == 4) {
-        const uint32_t *s = reinterpret_cast<const uint32_t *>(p);
-        r.q[0] = make_uint4(s[0], s[1], s[2], s[3]);
-        r.q[1] = make_uint4(s[4], s[5], s[6], s[7]);
+#pragma unroll
+        for (int i = 0; i < W; ++i) r.w[i] = reinterpret_cast<const uint32_t *>(p)[i];
     } else {
-        const uint16_t *s = reinterpret_cast<const uint16_t *>(p);
-        r.q[0] = make_uint4(s[0] | ((uint32_t)s[1] << 16), s[2] | ((uint32_t)s[3] << 16), s[4] | ((uint32_t)s[5] << 16), s[6] | ((uint32_t)s[7] << 16));
+#pragma unroll
+        for (int i = 0; i < W; ++i) r.w[i] = reinterpret_cast<const uint16_t *>(p)[2 * i] | ((uint32_t) reinterpret_cast<const uint16_t *>(p)[2 * i + 1] << 16);
     }
-    return r;
 }
 
+// The block's scale byte and its 32 codes. Magnitudes compare like their bit patterns, a NaN above infinity; 16-bit types
+// are compared two at a time.
 template <typename T>
-__device__ __forceinline__ void widen8(const Raw8<T> &r, float (&v)[8])
+__device__ __forceinline__ uint32_t encode_block(const RawBlock<T> &r, uint4 &codes)
 {
+    constexpr int W = RawBlock<T>::WORDS;
+    constexpr bool kHalf = std::is_same<T, __half>::value, kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    uint32_t top = 0;
     if constexpr (sizeof(T) == 4) {
-        v[0] = __uint_as_float(r.q[0].x); v[1] = __uint_as_float(r.q[0].y); v[2] = __uint_as_float(r.q[0].z); v[3] = __uint_as_float(r.q[0].w);
-        v[4] = __uint_as_float(r.q[1].x); v[5] = __uint_as_float(r.q[1].y); v[6] = __uint_as_float(r.q[1].z); v[7] = __uint_as_float(r.q[1].w);
+#pragma unroll
+        for (int i = 0; i < W; ++i) top = max(top, r.w[i] & 0x7FFFFFFFu);
     } else {
-        const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) m = __vmaxu2(m, r.w[i] & 0x7FFF7FFFu);
+        const uint32_t h = max(m & 0xFFFFu, m >> 16);
+        top = kHalf ? __float_as_uint(__half2float(__ushort_as_half((unsigned short)h))) : h << 16;
+    }
+    const uint32_t e = top >> 23;
+    uint32_t s = e > 2u ? e - 2u : 0u;
+    const float inv = __uint_as_float((254u - s) << 23); // 2^-X, a normal number for every s
+    uint32_t out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float v[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if constexpr (std::is_same<T, __half>::value) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                v[2 * i] = f.x;
-                v[2 * i + 1] = f.y;
+            if constexpr (kHalf) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r.w[4 * j + i]));
+                v[2 * i] = f.x * inv;
+                v[2 * i + 1] = f.y * inv;
+            } else if constexpr (kBf16) {
+                // Scaled two at a time in bf16, which has the exponents of fp32: the product with a power of two is exact, or
+                // so small that its code is 0 either way.
+                const __nv_bfloat162 p = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&r.w[4 * j + i]), __float2bfloat162_rn(inv));
+                const uint32_t q = *reinterpret_cast<const uint32_t *>(&p);
+                v[2 * i] = __uint_as_float(q << 16);
+                v[2 * i + 1] = __uint_as_float(q & 0xFFFF0000u);
             } else {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+                v[2 * i] = __uint_as_float(r.w[8 * j + 2 * i]) * inv;
+                v[2 * i + 1] = __uint_as_float(r.w[8 * j + 2 * i + 1]) * inv;
             }
         }
+        out[j] = mx_encode8(v);
     }
+    const bool finite = e != 255u; // else an infinity or a NaN
+    codes = finite ? make_uint4(out[0], out[1], out[2], out[3]) : make_uint4(0, 0, 0, 0);
+    return finite ? s : MX_NAN;
 }
 
-// One block of 128 rows x 128 k per CTA: its 512 bytes of scales are put together in shared memory and written whole.
-// Bound by memory: 2 + 17/32 bytes per value of a 16-bit type. A thread has the loads of four rows in flight.
-template <typename T>
-__global__ void __launch_bounds__(mxq::THREADS) mxfp4_quantize_kernel(const T *__restrict__ x, long long ldx, int vec, int groups, int rows, int K,
-                                                                      const int *offsets, uint8_t *__restrict__ packed,
-                                                                      uint8_t *__restrict__ scales, int *status)
+// Blocks of 128 rows x 128 k: their 512 bytes of scales are put together in shared memory and written whole. A thread takes
+// whole blocks of 32 values (64 bytes of a 16-bit type in, 16 bytes and a scale out): nothing is exchanged between
+// threads. The 256 threads lie across kAcross scale blocks of a slot (4 threads each) and 64 / kAcross rows: 4 for full slots, 16
+// for groups of a few rows, where most rows of a slot do not exist. A CTA takes `steps` times that many blocks, one
+// after the other, so that a large operand looks its rows up once for several.
+// Bound by memory (2 + 17/32 bytes per value of a 16-bit type). With eight values per thread, the largest magnitude by
+// shuffles and 4-byte stores the kernel was bound by instruction issue (109 instructions per eight values, 79 % of
+// the issue slots): 16384 x 11008 bf16 in 90 us.
+template <typename T, int kAcross>
+__global__ void __launch_bounds__(mxq::THREADS, sizeof(T) == 4 ? 3 : 4)
+mxfp4_quantize_kernel(const T *__restrict__ x, long long ldx, int vec, int groups, int rows, int K, int steps, const int *offsets,
+                      uint8_t *__restrict__ packed, uint8_t *__restrict__ scales, int *status)
 {
     using namespace mxq;
-    constexpr int BATCH = 4;
-    __shared__ __align__(16) uint8_t sc[MX_SCALE_BYTES];
-    const int chunks = mx_chunks(K);
-    const int slot = blockIdx.x / chunks, chunk = blockIdx.x - slot * chunks;
+    constexpr int BATCH = sizeof(T) == 4 ? 1 : 2, LINES = 64 / kAcross; // rows per pass
+    __shared__ __align__(16) uint8_t sc[2][kAcross * MX_SCALE_BYTES];
+    const int chunks = mx_chunks(K), per_cta = steps * kAcross, parts = (chunks + per_cta - 1) / per_cta;
+    const int slot = blockIdx.x / parts, part = blockIdx.x - slot * parts;
     // x may be what the kernel before writes and the output what it reads; once that is over, the product that follows
     // may set itself up.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const SlotRows s_rows = slot_rows(slot, offsets, groups, rows, status);
-    if (s_rows.first >= s_rows.end) return;
-    const int tr = threadIdx.x >> 4, tk = threadIdx.x & 15;
-    const int k = chunk * MX_CHUNK_K + tk * 8;
-#pragma unroll
-    for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
-        Raw8<T> raw[BATCH];
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int row = s_rows.first + (i0 + i) * ROWS + tr;
-            if (row < s_rows.end && k < K) raw[i] = load8(x + (long long)row * ldx + k, vec != 0); // K is a multiple of 32: a block's four threads agree
-            else raw[i] = {};
+    const int height = s_rows.end - s_rows.first;
+    if (height <= 0) return;
+    const int tr = threadIdx.x / (4 * kAcross), tk = threadIdx.x % (4 * kAcross);
+    const int chunk_end = min(chunks, (part + 1) * per_cta);
+    int half = 0;
+    for (int chunk = part * per_cta; chunk < chunk_end; chunk += kAcross, half ^= 1) {
+        uint8_t *scb = sc[half]; // the blocks before may still be on their way out of the other half
+        const int k = chunk * MX_CHUNK_K + tk * MX_BLOCK;
+        const bool whole = height == GROUP_SLOT_ROWS && (chunk + kAcross) * MX_CHUNK_K <= K;
+        if (!whole) { // bytes outside the matrix are 0
+            for (int i = threadIdx.x; i < kAcross * MX_SCALE_BYTES / 16; i += THREADS) reinterpret_cast<uint4 *>(scb)[i] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
         }
+        const T *src = x + (long long)(s_rows.first + tr) * ldx + k;
+        uint8_t *dst = packed + (long long)(s_rows.first + tr) * (K / 2) + (k >> 1);
+#pragma unroll 1
+        for (int r0 = 0; r0 < height; r0 += BATCH * LINES) {
+            RawBlock<T> raw[BATCH];
+            bool in[BATCH];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int r = (i0 + i) * ROWS + tr, row = s_rows.first + r;
-            float v[8];
-            widen8(raw[i], v);
-            uint32_t top = 0; // largest magnitude as an integer: ordered like the values, NaN above infinity
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const uint32_t e = top >> 23;
-            uint32_t s = e > 2u ? e - 2u : 0u;
-            float inv = __uint_as_float((254u - s) << 23); // 2^-X, a normal number for every s
-            if (e == 255u) {
-                s = MX_NAN;
-                inv = 0.0f;
+            for (int i = 0; i < BATCH; ++i) {
+                in[i] = whole || (r0 + i * LINES + tr < height && k < K);
+                if (in[i]) load_block(raw[i], src + (long long)(r0 + i * LINES) * ldx, vec);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = e == 255u ? 0.0f : v[j] * inv;
-            if (row < s_rows.end && k < K) *reinterpret_cast<uint32_t *>(packed + (long long)row * (K / 2) + (k >> 1)) = mx_encode8(v);
-            if ((tk & 3) == 0) sc[mx_scale_at(r, tk >> 2)] = (uint8_t)s; // 0 outside the matrix
+            for (int i = 0; i < BATCH; ++i) {
+                if (!in[i]) continue;
+                uint4 codes;
+                const uint32_t s = encode_block(raw[i], codes);
+                *reinterpret_cast<uint4 *>(dst + (long long)(r0 + i * LINES) * (K / 2)) = codes;
+                scb[(tk >> 2) * MX_SCALE_BYTES + mx_scale_at(r0 + i * LINES + tr, tk & 3)] = (uint8_t)s;
+            }
         }
+        __syncthreads();
+        const int left = (chunk_end - chunk < kAcross ? chunk_end - chunk : kAcross) * MX_SCALE_BYTES / 16;
+        for (int i = threadIdx.x; i < left; i += THREADS)
+            reinterpret_cast<uint4 *>(scales + ((long long)slot * chunks + chunk) * MX_SCALE_BYTES)[i] = reinterpret_cast<const uint4 *>(scb)[i];
     }
-    __syncthreads();
-    if (threadIdx.x < MX_SCALE_BYTES / 16)
-        reinterpret_cast<uint4 *>(scales + ((long long)slot * chunks + chunk) * MX_SCALE_BYTES)[threadIdx.x] = reinterpret_cast<const uint4 *>(sc)[threadIdx.x];
 }
 
 template <typename T>
@@ -232,7 +277,7 @@ __global__ void __launch_bounds__(mxq::THREADS) mxfp4_dequant_kernel(const uint8
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
         const int row = s_rows.first + i * ROWS + tr;
-        if (row >= s_rows.end) continue;
+        if (row >= s_rows.end) break;
         const float s = mx_scale_value(scale[i]);
         uint32_t h[4];
         mx_decode8(codes[i], h);
@@ -254,13 +299,9 @@ __global__ void __launch_bounds__(mxq::THREADS) mxfp4_dequant_kernel(const uint8
     }
 }
 
-static int slot_grid(int groups, int rows, int K, const int *offsets, unsigned *grid)
+static long long slot_count(int groups, int rows, const int *offsets)
 {
-    const long long slots = offsets ? grouped_slot_bound(groups, rows) : (long long)groups * (((rows / groups) + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS);
-    const long long blocks = slots * mx_chunks(K);
-    if (blocks > 0x7FFFFFFFLL) return set_error(BTM_ERR_UNSUPPORTED, "mxfp4: operand too large (%lld scale blocks)", blocks);
-    *grid = (unsigned)blocks;
-    return BTM_OK;
+    return offsets ? grouped_slot_bound(groups, rows) : (long long)groups * (((rows / groups) + GROUP_SLOT_ROWS - 1) / GROUP_SLOT_ROWS);
 }
 
 // Programmatic stream serialisation: the kernels wait for their predecessor by themselves.
@@ -280,28 +321,38 @@ static cudaError_t launch_pdl(void (*kernel)(P...), unsigned grid, cudaStream_t 
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
+template <typename T>
+static int quantize_as(cudaStream_t st, int groups, int rows, int K, const int *offsets, const void *x, long long ldx, void *packed, void *scales, int *status)
+{
+    const long long slots = slot_count(groups, rows, offsets), chunks = mx_chunks(K);
+    const bool flat = getenv("BTM_FLAT") ? atoi(getenv("BTM_FLAT")) : rows <= 16LL * groups;
+    const int across = flat ? 1 : 4;
+    // More than one step per CTA once there are several waves of them (four CTAs per SM).
+    long long steps = slots * chunks / (across * 4LL * 4 * 148);
+    steps = steps < 1 ? 1 : steps > 8 ? 8 : steps;
+    const long long blocks = slots * ((chunks + steps * across - 1) / (steps * across));
+    if (blocks > 0x7FFFFFFFLL) return set_error(BTM_ERR_UNSUPPORTED, "mxfp4 quantise: operand too large (%lld scale blocks)", slots * chunks);
+    const long long pitch = ldx * (long long)sizeof(T);
+    const int vec = (((uintptr_t)x | (uintptr_t)pitch) & 31) == 0 ? 2 : (((uintptr_t)x | (uintptr_t)pitch) & 15) == 0 ? 1 : 0;
+    const cudaError_t e = launch_pdl(flat ? mxfp4_quantize_kernel<T, 1> : mxfp4_quantize_kernel<T, 4>, (unsigned)blocks, st, (const T *)x, ldx, vec, groups,
+                                     rows, K, (int)steps, offsets, (uint8_t *)packed, (uint8_t *)scales, status);
+    return check_cuda(e, "mxfp4 quantise launch");
+}
+
 int launch_mxfp4_quantize(cudaStream_t st, int src_dtype, int groups, int rows, int K, const int *offsets, const void *x, long long ldx,
                           void *packed, void *scales, int *status)
 {
-    unsigned grid;
-    if (int rc = slot_grid(groups, rows, K, offsets, &grid)) return rc;
-    if (grid == 0) return BTM_OK;
-    const int es = src_dtype == BTM_F32 ? 4 : 2;
-    const int vec = ((uintptr_t)x & 15) == 0 && (ldx * es) % 16 == 0;
-    uint8_t *pk = (uint8_t *)packed, *sc = (uint8_t *)scales;
-    cudaError_t e;
-    if (src_dtype == BTM_F32) e = launch_pdl(mxfp4_quantize_kernel<float>, grid, st, (const float *)x, ldx, vec, groups, rows, K, offsets, pk, sc, status);
-    else if (src_dtype == BTM_F16) e = launch_pdl(mxfp4_quantize_kernel<__half>, grid, st, (const __half *)x, ldx, vec, groups, rows, K, offsets, pk, sc, status);
-    else e = launch_pdl(mxfp4_quantize_kernel<__nv_bfloat16>, grid, st, (const __nv_bfloat16 *)x, ldx, vec, groups, rows, K, offsets, pk, sc, status);
-    return check_cuda(e, "mxfp4 quantise launch");
+    if (src_dtype == BTM_F32) return quantize_as<float>(st, groups, rows, K, offsets, x, ldx, packed, scales, status);
+    if (src_dtype == BTM_F16) return quantize_as<__half>(st, groups, rows, K, offsets, x, ldx, packed, scales, status);
+    return quantize_as<__nv_bfloat16>(st, groups, rows, K, offsets, x, ldx, packed, scales, status);
 }
 
 int launch_mxfp4_dequant(cudaStream_t st, int dst_dtype, int groups, int rows, int K, const int *offsets, const void *packed,
                          const void *scales, void *out, long long ldo, int *status)
 {
-    unsigned grid;
-    if (int rc = slot_grid(groups, rows, K, offsets, &grid)) return rc;
-    if (grid == 0) return BTM_OK;
+    const long long blocks = slot_count(groups, rows, offsets) * mx_chunks(K);
+    if (blocks > 0x7FFFFFFFLL) return set_error(BTM_ERR_UNSUPPORTED, "mxfp4 dequantise: operand too large (%lld scale blocks)", blocks);
+    const unsigned grid = (unsigned)blocks;
     const int es = dst_dtype == BTM_F32 ? 4 : 2;
     const int vec = ((uintptr_t)out & 15) == 0 && (ldo * es) % 16 == 0;
     const uint8_t *pk = (const uint8_t *)packed, *sc = (const uint8_t *)scales;
