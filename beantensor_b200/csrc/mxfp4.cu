@@ -5,7 +5,6 @@
 // is exact, so the only rounding is the one to four bits. A block that holds an infinity or a NaN has no such scale: it
 // gets scale 255 (NaN) and zero codes, and everything that it enters becomes NaN. Dequantise: q 2^X, rounded once.
 #include <cstring>
-#include <cstdlib>
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -179,8 +178,8 @@ __device__ __forceinline__ uint32_t encode_block(const RawBlock<T> &r, uint4 &co
 
 // Blocks of 128 rows x 128 k: their 512 bytes of scales are put together in shared memory and written whole. A thread takes
 // whole blocks of 32 values (64 bytes of a 16-bit type in, 16 bytes and a scale out): nothing is exchanged between
-// threads. The 256 threads lie across kAcross scale blocks of a slot (4 threads each) and 64 / kAcross rows: 4 for full slots, 16
-// for groups of a few rows, where most rows of a slot do not exist. A CTA takes `steps` times that many blocks, one
+// threads. The 256 threads lie across kAcross scale blocks of a slot (4 threads each) and 64 / kAcross rows (quantize_as
+// chooses). A CTA takes `steps` times that many blocks, one
 // after the other, so that a large operand looks its rows up once for several.
 // Bound by memory (2 + 17/32 bytes per value of a 16-bit type). With eight values per thread, the largest magnitude by
 // shuffles and 4-byte stores the kernel was bound by instruction issue (109 instructions per eight values, 79 % of
@@ -325,8 +324,10 @@ template <typename T>
 static int quantize_as(cudaStream_t st, int groups, int rows, int K, const int *offsets, const void *x, long long ldx, void *packed, void *scales, int *status)
 {
     const long long slots = slot_count(groups, rows, offsets), chunks = mx_chunks(K);
-    const bool flat = getenv("BTM_FLAT") ? atoi(getenv("BTM_FLAT")) : rows <= 16LL * groups;
-    const int across = flat ? 1 : 4;
+    // One block across, 64 rows at a time, while all CTAs are resident at once (four per SM): then the time is a CTA's latency.
+    // Four across, 16 rows at a time, beyond. Measured, one / four: 256 x 2048 plain (32 CTAs at one) 2.4 / 4.7 us, 3001 x 1440 in 24
+    // groups (564) 4.7 / 6.6; 256 x 2048 in 64 groups (1040) 5.1 / 2.8, 2048 x 4096 in 64 (2560) 12.0 / 6.7, 16384 x 11008 71.0 / 69.7.
+    const int across = slots * chunks <= 4 * 148 ? 1 : 4;
     // More than one step per CTA once there are several waves of them (four CTAs per SM).
     long long steps = slots * chunks / (across * 4LL * 4 * 148);
     steps = steps < 1 ? 1 : steps > 8 ? 8 : steps;
@@ -334,7 +335,7 @@ static int quantize_as(cudaStream_t st, int groups, int rows, int K, const int *
     if (blocks > 0x7FFFFFFFLL) return set_error(BTM_ERR_UNSUPPORTED, "mxfp4 quantise: operand too large (%lld scale blocks)", slots * chunks);
     const long long pitch = ldx * (long long)sizeof(T);
     const int vec = (((uintptr_t)x | (uintptr_t)pitch) & 31) == 0 ? 2 : (((uintptr_t)x | (uintptr_t)pitch) & 15) == 0 ? 1 : 0;
-    const cudaError_t e = launch_pdl(flat ? mxfp4_quantize_kernel<T, 1> : mxfp4_quantize_kernel<T, 4>, (unsigned)blocks, st, (const T *)x, ldx, vec, groups,
+    const cudaError_t e = launch_pdl(across == 1 ? mxfp4_quantize_kernel<T, 1> : mxfp4_quantize_kernel<T, 4>, (unsigned)blocks, st, (const T *)x, ldx, vec, groups,
                                      rows, K, (int)steps, offsets, (uint8_t *)packed, (uint8_t *)scales, status);
     return check_cuda(e, "mxfp4 quantise launch");
 }

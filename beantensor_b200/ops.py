@@ -188,14 +188,34 @@ def quantize_int4_gpu(w: torch.Tensor, w_packed: torch.Tensor, scales: torch.Ten
     raise_for_status(rc)
 
 
-def _offsets(offsets: torch.Tensor, groups: int, what: str) -> None:
-    if offsets.dtype != torch.int32 or offsets.dim() != 1 or not offsets.is_contiguous() or offsets.shape[0] != groups + 1:
-        raise ValueError(f"{what}: offsets must be a contiguous Int32 tensor of groups + 1 entries")
+# The grouped and microscaled operators sit in front of kernels of a few microseconds: their guards look at each tensor once
+# and cost little; whatever fails goes through the slower functions that find out why and raise.
+_U8, _I32 = torch.uint8, torch.int32
+_DT16 = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _pitch(t: torch.Tensor) -> int:
-    """Leading dimension of a row-major matrix (the last two dimensions of t); a single row has none of its own."""
-    return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], 1)
+def _same_gpu(*tensors: torch.Tensor) -> None:
+    """Raises with the operator boundary's messages; called when the tensors are not all on one GPU."""
+    _require_gpu(*tensors)
+    raise ValueError("Tensors live on different GPUs")
+
+
+def _not_supported(what: str, dtype) -> None:
+    from .errors import NotImplementedOp
+    raise NotImplementedOp(f"{what}: dtype {dtype} is not supported")
+
+
+def _bad_offsets(what: str) -> None:
+    raise ValueError(f"{what}: offsets must be a contiguous Int32 tensor of groups + 1 entries")
+
+
+def _row_pitch(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
+    """Leading dimension of a row-major matrix, the last two dimensions of t; a single row has none of its own."""
+    st = t.stride()
+    if cols > 1 and st[-1] != 1:
+        raise ValueError(f"{name} must be row-major (last stride 1)")  # Tensor/Tensor.cpp:157-162
+    return st[-2] if rows > 1 else (cols or 1)
 
 
 def grouped_matmul_gpu(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor) -> None:
@@ -205,99 +225,125 @@ def grouped_matmul_gpu(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, 
     b.transpose(1, 2) and the output gradient as `a` this is the gradient of the activations. Rows outside the groups
     keep what `out` held.
     """
-    dev = _require_gpu(a, b, offsets, out)
-    if a.dim() != 2 or b.dim() != 3 or out.dim() != 2:
+    dev = out.get_device()
+    if dev < 0 or a.get_device() != dev or b.get_device() != dev or offsets.get_device() != dev:
+        _same_gpu(a, b, offsets, out)
+    sa, sb = a.shape, b.shape
+    if len(sa) != 2 or len(sb) != 3 or out.dim() != 2:
         raise ValueError("grouped_matmul_gpu takes a 2-D, b 3-D and out 2-D")
-    if a.dtype != b.dtype or a.dtype != out.dtype:
+    dtype = a.dtype
+    if b.dtype != dtype or out.dtype != dtype:
         raise ValueError("grouped_matmul_gpu: dtypes differ")
-    if a.dtype not in (torch.float16, torch.bfloat16):
-        from .errors import NotImplementedOp
-        raise NotImplementedOp(f"grouped_matmul_gpu: dtype {a.dtype} is not supported")
-    rows, K = a.shape
-    G, K2, N = b.shape
+    dt = _DT16.get(dtype)
+    if dt is None:
+        _not_supported("grouped_matmul_gpu", dtype)
+    rows, K = sa
+    G, K2, N = sb
     if K != K2 or out.shape != (rows, N):
-        raise ValueError(f"grouped_matmul_gpu: shape mismatch {tuple(a.shape)} x {tuple(b.shape)} -> {tuple(out.shape)}")
-    _offsets(offsets, G, "grouped_matmul_gpu")
-    _rowmajor(a, "a")
-    _rowmajor(out, "out")
-    trans = not (b.stride(2) == 1 or N <= 1)
-    if trans and not (b.stride(1) == 1 or K <= 1):
+        raise ValueError(f"grouped_matmul_gpu: shape mismatch {tuple(sa)} x {tuple(sb)} -> {tuple(out.shape)}")
+    if offsets.dtype != _I32 or offsets.shape != (G + 1,) or not offsets.is_contiguous():
+        _bad_offsets("grouped_matmul_gpu")
+    lda, ldc = _row_pitch(a, rows, K, "a"), _row_pitch(out, rows, N, "out")
+    bg, bk, bn = b.stride()
+    trans = bn != 1 and N > 1
+    if not trans:
+        ldb, outer = (bk if K > 1 else N or 1), K
+    elif bk == 1 or K <= 1:
+        ldb, outer = (bn if N > 1 else K or 1), N
+    else:
         raise ValueError("grouped_matmul_gpu: each matrix of b must be row-major or transposed row-major")
-    bt = b.transpose(1, 2) if trans else b
-    ldb = _pitch(bt)
-    rc = _LIB().btm_gemm_grouped(dev, _stream(dev), _DT[a.dtype], G, rows, N, K, offsets.data_ptr(), a.data_ptr(), _pitch(a), b.data_ptr(),
-                                 b.stride(0) if G > 1 else bt.shape[1] * ldb, ldb, 1 if trans else 0, out.data_ptr(), _pitch(out))
-    raise_for_status(rc)
+    rc = _LIB().btm_gemm_grouped(dev, _raw_stream(dev), dt, G, rows, N, K, offsets.data_ptr(), a.data_ptr(), lda, b.data_ptr(),
+                                 bg if G > 1 else outer * ldb, ldb, 1 if trans else 0, out.data_ptr(), ldc)
+    if rc:
+        raise_for_status(rc)
 
 
 def grouped_matmul_wgrad_gpu(a: torch.Tensor, dout: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor) -> None:
     """The weight gradient of grouped_matmul_gpu: out[g] = a[rows of g]^T . dout[rows of g], zero for an empty group.
 
     a [rows,K], dout [rows,N], out [groups,K,N], fp16/bf16 with fp32 accumulation."""
-    dev = _require_gpu(a, dout, offsets, out)
-    if a.dim() != 2 or dout.dim() != 2 or out.dim() != 3:
+    dev = out.get_device()
+    if dev < 0 or a.get_device() != dev or dout.get_device() != dev or offsets.get_device() != dev:
+        _same_gpu(a, dout, offsets, out)
+    sa, sd = a.shape, dout.shape
+    if len(sa) != 2 or len(sd) != 2 or out.dim() != 3:
         raise ValueError("grouped_matmul_wgrad_gpu takes a 2-D, dout 2-D and out 3-D")
-    if a.dtype != dout.dtype or a.dtype != out.dtype:
+    dtype = a.dtype
+    if dout.dtype != dtype or out.dtype != dtype:
         raise ValueError("grouped_matmul_wgrad_gpu: dtypes differ")
-    if a.dtype not in (torch.float16, torch.bfloat16):
-        from .errors import NotImplementedOp
-        raise NotImplementedOp(f"grouped_matmul_wgrad_gpu: dtype {a.dtype} is not supported")
-    rows, K = a.shape
-    rows2, N = dout.shape
-    G = out.shape[0]
-    if rows != rows2 or out.shape != (G, K, N):
-        raise ValueError(f"grouped_matmul_wgrad_gpu: shape mismatch {tuple(a.shape)} x {tuple(dout.shape)} -> {tuple(out.shape)}")
-    _offsets(offsets, G, "grouped_matmul_wgrad_gpu")
-    for t, name in ((a, "a"), (dout, "dout"), (out, "out")):
-        _rowmajor(t, name)
-    ldc = _pitch(out)
-    rc = _LIB().btm_gemm_grouped_wgrad(dev, _stream(dev), _DT[a.dtype], G, rows, K, N, offsets.data_ptr(), a.data_ptr(), _pitch(a),
-                                       dout.data_ptr(), _pitch(dout), out.data_ptr(), out.stride(0) if G > 1 else K * ldc, ldc)
-    raise_for_status(rc)
+    dt = _DT16.get(dtype)
+    if dt is None:
+        _not_supported("grouped_matmul_wgrad_gpu", dtype)
+    rows, K = sa
+    rows2, N = sd
+    G, Ko, No = out.shape
+    if rows != rows2 or Ko != K or No != N:
+        raise ValueError(f"grouped_matmul_wgrad_gpu: shape mismatch {tuple(sa)} x {tuple(sd)} -> {tuple(out.shape)}")
+    if offsets.dtype != _I32 or offsets.shape != (G + 1,) or not offsets.is_contiguous():
+        _bad_offsets("grouped_matmul_wgrad_gpu")
+    lda, ldd, ldc = _row_pitch(a, rows, K, "a"), _row_pitch(dout, rows, N, "dout"), _row_pitch(out, K, N, "out")
+    rc = _LIB().btm_gemm_grouped_wgrad(dev, _raw_stream(dev), dt, G, rows, K, N, offsets.data_ptr(), a.data_ptr(), lda, dout.data_ptr(), ldd,
+                                       out.data_ptr(), out.stride(0) if G > 1 else K * ldc, ldc)
+    if rc:
+        raise_for_status(rc)
 
 
 def mxfp4_scale_bytes(rows: int, K: int, groups: int = 1) -> int:
-    """Bytes that hold the scales of `rows` microscaled rows of K values in `groups` groups, however the rows are divided."""
-    return _LIB().btm_mxfp4_scale_bytes(groups, rows, K)
+    """Bytes that hold the scales of `rows` microscaled rows of K values in `groups` groups, however the rows are divided
+    (btm_mxfp4_scale_bytes)."""
+    if rows <= 0 or K <= 0 or groups <= 0:
+        return 0
+    return (rows + 127 * (groups if groups < rows else rows)) // 128 * ((K + 127) // 128) * 512
 
 
-def _mxfp4_operand(packed: torch.Tensor, scales: torch.Tensor, rows: int, K: int, groups: int, scale_bytes: int, what: str) -> None:
-    if packed.dtype != torch.uint8 or scales.dtype != torch.uint8:
+def _bad_mxfp4(packed: torch.Tensor, scales: torch.Tensor, K: int, what: str, fits: bool = True) -> None:
+    """Raises: why packed values and scales do not fit the operator."""
+    if packed.dtype != _U8 or scales.dtype != _U8:
         raise ValueError(f"{what}: packed values and scales are bytes")
     if K % 32:
         raise ValueError(f"{what}: K={K} must be a multiple of 32")
-    if packed.numel() != rows * (K // 2) or scales.numel() < scale_bytes:
+    if not fits:
         raise ValueError(f"{what}: shape mismatch")
-    if not (packed.is_contiguous() and scales.is_contiguous()):
-        raise ValueError(f"{what}: packed values and scales must be contiguous")
+    raise ValueError(f"{what}: packed values and scales must be contiguous")
 
 
-def _mxfp4_convert(x, packed, scales, offsets, what: str):
-    """Checks shared by quantize_mxfp4_gpu and dequant_mxfp4_gpu; x is the plain side. Returns the C arguments."""
-    tensors = (x, packed, scales) if offsets is None else (x, packed, scales, offsets)
-    dev = _require_gpu(*tensors)
-    if x.dtype not in _DT:
-        from .errors import NotImplementedOp
-        raise NotImplementedOp(f"{what}: dtype {x.dtype} is not supported")
-    if x.dim() not in (2, 3) or packed.shape[:-1] != x.shape[:-1] or packed.shape[-1] * 2 != x.shape[-1]:
-        raise ValueError(f"{what}: shape mismatch {tuple(x.shape)} and {tuple(packed.shape)}")
-    K = x.shape[-1]
-    if x.dim() == 3:
+def _mxfp4_convert(fn, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor | None, what: str, quantize: bool) -> None:
+    """quantize_mxfp4_gpu and dequant_mxfp4_gpu; x is the plain side."""
+    dev = x.get_device()
+    if dev < 0 or packed.get_device() != dev or scales.get_device() != dev or (offsets is not None and offsets.get_device() != dev):
+        _same_gpu(*((x, packed, scales) if offsets is None else (x, packed, scales, offsets)))
+    dt = _DT.get(x.dtype)
+    if dt is None:
+        _not_supported(what, x.dtype)
+    shape = x.shape
+    if len(shape) == 2:
+        rows, K = shape
+        ld = _row_pitch(x, rows, K, "the matrix")
+        if offsets is None:
+            groups, table = 1, None
+        else:
+            groups, table = offsets.numel() - 1, offsets.data_ptr()
+            if offsets.dtype != _I32 or offsets.dim() != 1 or groups < 0 or not offsets.is_contiguous():
+                _bad_offsets(what)
+        fits = packed.shape == (rows, K // 2) and scales.numel() >= mxfp4_scale_bytes(rows, K, groups)
+    elif len(shape) == 3:
         if offsets is not None:
             raise ValueError(f"{what}: offsets go with 2-D tensors; the groups of a 3-D one are its first dimension")
         if not x.is_contiguous():
             raise ValueError(f"{what}: a 3-D tensor must be contiguous")
-        groups, rows, ld = x.shape[0], x.shape[0] * x.shape[1], K
-        need = groups * mxfp4_scale_bytes(x.shape[1], K)
+        groups, N, K = shape
+        rows, ld, table = groups * N, K, None
+        fits = packed.shape == (groups, N, K // 2) and scales.numel() >= groups * mxfp4_scale_bytes(N, K)
     else:
-        _rowmajor(x, "the matrix")
-        rows, ld = x.shape[0], _pitch(x)
-        groups = 1 if offsets is None else offsets.shape[0] - 1
-        if offsets is not None:
-            _offsets(offsets, groups, what)
-        need = mxfp4_scale_bytes(rows, K, groups)
-    _mxfp4_operand(packed, scales, rows, K, groups, need, what)
-    return dev, groups, rows, K, max(ld, K), None if offsets is None else offsets.data_ptr()
+        raise ValueError(f"{what} takes 2-D or 3-D tensors")
+    if not fits or K % 32 or packed.dtype != _U8 or scales.dtype != _U8 or not packed.is_contiguous() or not scales.is_contiguous():
+        _bad_mxfp4(packed, scales, K, what, fits)
+    if quantize:
+        rc = fn(dev, _raw_stream(dev), dt, groups, rows, K, table, x.data_ptr(), ld, packed.data_ptr(), scales.data_ptr())
+    else:
+        rc = fn(dev, _raw_stream(dev), dt, groups, rows, K, table, packed.data_ptr(), scales.data_ptr(), x.data_ptr(), ld)
+    if rc:
+        raise_for_status(rc)
 
 
 def quantize_mxfp4_gpu(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor | None = None) -> None:
@@ -307,58 +353,67 @@ def quantize_mxfp4_gpu(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tens
     (what grouped_matmul_mxfp4_gpu takes). x [groups,N,K] -> packed [groups,N,K/2], the weights of all experts.
     scales: mxfp4_scale_bytes(rows, K, groups) bytes, or groups * mxfp4_scale_bytes(N, K) for a 3-D x, in the block
     order that include/btm.h defines."""
-    dev, groups, rows, K, ld, offs = _mxfp4_convert(x, packed, scales, offsets, "quantize_mxfp4_gpu")
-    rc = _LIB().btm_mxfp4_quantize(dev, _stream(dev), _DT[x.dtype], groups, rows, K, offs, x.data_ptr(), ld, packed.data_ptr(), scales.data_ptr())
-    raise_for_status(rc)
+    _mxfp4_convert(_LIB().btm_mxfp4_quantize, x, packed, scales, offsets, "quantize_mxfp4_gpu", True)
 
 
 def dequant_mxfp4_gpu(packed: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, offsets: torch.Tensor | None = None) -> None:
     """The values that quantize_mxfp4_gpu's output stands for, rounded once to out's dtype; shapes as there."""
-    dev, groups, rows, K, ld, offs = _mxfp4_convert(out, packed, scales, offsets, "dequant_mxfp4_gpu")
-    rc = _LIB().btm_mxfp4_dequant(dev, _stream(dev), _DT[out.dtype], groups, rows, K, offs, packed.data_ptr(), scales.data_ptr(), out.data_ptr(), ld)
-    raise_for_status(rc)
+    _mxfp4_convert(_LIB().btm_mxfp4_dequant, out, packed, scales, offsets, "dequant_mxfp4_gpu", False)
 
 
-def _mxfp4_out(out: torch.Tensor, what: str) -> None:
-    if out.dtype not in (torch.float16, torch.bfloat16):
-        from .errors import NotImplementedOp
-        raise NotImplementedOp(f"{what}: output dtype {out.dtype} is not supported")
-    _rowmajor(out, "out")
+def _mxfp4_product_dtype(what: str, act, act_scales, w, w_scales, out, K: int) -> int:
+    dt = _DT16.get(out.dtype)
+    if dt is None:
+        _not_supported(what, out.dtype)
+    if act.dtype != _U8 or act_scales.dtype != _U8 or not act.is_contiguous() or not act_scales.is_contiguous() or K % 32:
+        _bad_mxfp4(act, act_scales, K, what)
+    if w.dtype != _U8 or w_scales.dtype != _U8 or not w.is_contiguous() or not w_scales.is_contiguous():
+        _bad_mxfp4(w, w_scales, K, what)
+    return dt
 
 
 def matmul_mxfp4_gpu(act: torch.Tensor, act_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> None:
     """out[M,N] = act[M,K] . w[N,K]^T for operands that quantize_mxfp4_gpu wrote (packed [.., K/2]); out fp16/bf16."""
-    dev = _require_gpu(act, act_scales, w, w_scales, out)
-    if act.dim() != 2 or w.dim() != 2 or out.dim() != 2:
+    dev = out.get_device()
+    if dev < 0 or act.get_device() != dev or act_scales.get_device() != dev or w.get_device() != dev or w_scales.get_device() != dev:
+        _same_gpu(act, act_scales, w, w_scales, out)
+    sa, sw = act.shape, w.shape
+    if len(sa) != 2 or len(sw) != 2 or out.dim() != 2:
         raise ValueError("matmul_mxfp4_gpu takes 2-D operands")
-    M, K, N = act.shape[0], act.shape[1] * 2, w.shape[0]
-    if w.shape[1] * 2 != K or out.shape != (M, N):
+    M, half = sa
+    N, half2 = sw
+    K = 2 * half
+    if half != half2 or out.shape != (M, N) or act_scales.numel() < mxfp4_scale_bytes(M, K) or w_scales.numel() < mxfp4_scale_bytes(N, K):
         raise ValueError("matmul_mxfp4_gpu: shape mismatch")
-    _mxfp4_operand(act, act_scales, M, K, 1, mxfp4_scale_bytes(M, K), "matmul_mxfp4_gpu")
-    _mxfp4_operand(w, w_scales, N, K, 1, mxfp4_scale_bytes(N, K), "matmul_mxfp4_gpu")
-    _mxfp4_out(out, "matmul_mxfp4_gpu")
-    rc = _LIB().btm_mxfp4_matmul(dev, _stream(dev), _DT[out.dtype], M, N, K, act.data_ptr(), act_scales.data_ptr(), w.data_ptr(),
-                                 w_scales.data_ptr(), out.data_ptr(), _pitch(out))
-    raise_for_status(rc)
+    dt = _mxfp4_product_dtype("matmul_mxfp4_gpu", act, act_scales, w, w_scales, out, K)
+    rc = _LIB().btm_mxfp4_matmul(dev, _raw_stream(dev), dt, M, N, K, act.data_ptr(), act_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(),
+                                 out.data_ptr(), _row_pitch(out, M, N, "out"))
+    if rc:
+        raise_for_status(rc)
 
 
 def grouped_matmul_mxfp4_gpu(act: torch.Tensor, act_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, offsets: torch.Tensor,
                              out: torch.Tensor) -> None:
     """out[r] = act[r] . w[g]^T for the rows r of group g; act [rows,K/2] quantised with these offsets, w [groups,N,K/2]."""
-    dev = _require_gpu(act, act_scales, w, w_scales, offsets, out)
-    if act.dim() != 2 or w.dim() != 3 or out.dim() != 2:
+    dev = out.get_device()
+    if (dev < 0 or act.get_device() != dev or act_scales.get_device() != dev or w.get_device() != dev or w_scales.get_device() != dev
+            or offsets.get_device() != dev):
+        _same_gpu(act, act_scales, w, w_scales, offsets, out)
+    sa, sw = act.shape, w.shape
+    if len(sa) != 2 or len(sw) != 3 or out.dim() != 2:
         raise ValueError("grouped_matmul_mxfp4_gpu takes act 2-D, w 3-D and out 2-D")
-    rows, K = act.shape[0], act.shape[1] * 2
-    G, N = w.shape[0], w.shape[1]
-    if w.shape[2] * 2 != K or out.shape != (rows, N):
+    rows, half = sa
+    G, N, half2 = sw
+    K = 2 * half
+    if half != half2 or out.shape != (rows, N) or act_scales.numel() < mxfp4_scale_bytes(rows, K, G) or w_scales.numel() < G * mxfp4_scale_bytes(N, K):
         raise ValueError("grouped_matmul_mxfp4_gpu: shape mismatch")
-    _offsets(offsets, G, "grouped_matmul_mxfp4_gpu")
-    _mxfp4_operand(act, act_scales, rows, K, G, mxfp4_scale_bytes(rows, K, G), "grouped_matmul_mxfp4_gpu")
-    _mxfp4_operand(w, w_scales, G * N, K, G, G * mxfp4_scale_bytes(N, K), "grouped_matmul_mxfp4_gpu")
-    _mxfp4_out(out, "grouped_matmul_mxfp4_gpu")
-    rc = _LIB().btm_mxfp4_matmul_grouped(dev, _stream(dev), _DT[out.dtype], G, rows, N, K, offsets.data_ptr(), act.data_ptr(),
-                                         act_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), _pitch(out))
-    raise_for_status(rc)
+    if offsets.dtype != _I32 or offsets.shape != (G + 1,) or not offsets.is_contiguous():
+        _bad_offsets("grouped_matmul_mxfp4_gpu")
+    dt = _mxfp4_product_dtype("grouped_matmul_mxfp4_gpu", act, act_scales, w, w_scales, out, K)
+    rc = _LIB().btm_mxfp4_matmul_grouped(dev, _raw_stream(dev), dt, G, rows, N, K, offsets.data_ptr(), act.data_ptr(), act_scales.data_ptr(),
+                                         w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), _row_pitch(out, rows, N, "out"))
+    if rc:
+        raise_for_status(rc)
 
 
 def convert_gpu(src: torch.Tensor, dst: torch.Tensor) -> None:

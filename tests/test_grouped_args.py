@@ -127,3 +127,11 @@ def test_cpu_tensors_are_refused():
         ops.quantize_mxfp4_gpu(a, by[:64].reshape(4, 16), by)
     with pytest.raises(GPUTaskOnCPUBuild):
         ops.matmul_mxfp4_gpu(by[:64].reshape(4, 16), by, by[:256].reshape(16, 16), by, out)
+
+
+def test_scale_bytes_of_both_sides_agree():
+    n = _lib.lib().btm_mxfp4_scale_bytes
+    for groups in (0, 1, 2, 7, 64, 300):
+        for rows in (0, 1, 5, 127, 128, 129, 1000, 2 ** 31 - 1):
+            for K in (0, 32, 128, 160, 4096):
+                assert ops.mxfp4_scale_bytes(rows, K, groups) == n(groups, rows, K)
