@@ -140,7 +140,8 @@ int configure_mxfp4_kernels();
 int configure_mxfp4_pair_kernels();
 int launch_mxfp4_decode(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *status);
 int launch_mxfp4_matmul_pair(const Mxfp4Call &c, cudaStream_t st, int sm_count, const GemmParams &p, const CUtensorMap &tmA, const CUtensorMap &tmA_band,
-                             const CUtensorMap &tmC);
+                             const CUtensorMap &sfa, const CUtensorMap &sfb, const CUtensorMap &tmC);
+int encode_mx_scales(CUtensorMap *m, const void *scales, int K, uint64_t blocks, uint64_t groups, uint32_t box_rows);
 int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *status);
 // Fills `cm` for the destinations in `p` (no-op when p.c_vec_ok == 0: the general store path needs no maps).
 int encode_store_maps(StoreMaps *cm, int dtype, const GemmParams &p);

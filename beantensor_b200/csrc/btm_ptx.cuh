@@ -232,13 +232,6 @@ __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap *m, int x, int
 {
     asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(m), "r"(x), "r"(y), "r"(z) : "memory");
 }
-// Untiled bulk copy global -> this CTA's shared memory; addresses and size are multiples of 16 bytes.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
-                 "r"(bar)
-                 : "memory");
-}
 
 // ---------------------------------------------------------------- CTA pairs
 __device__ __forceinline__ uint32_t pair_rank()

@@ -419,11 +419,11 @@ int launch_mxfp4_decode(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
     int rc = prepare(&a, c.rows, c.groups, c.N, c.K, c.offsets, c.out, c.ldo, status, sm_count, true, &split, &blocks);
     if (rc) return rc;
     DecodeMaps maps;
-    const uint64_t pitch = (uint64_t)c.K / 2, words = (uint64_t)mx_chunks(c.K) * (MX_SCALE_BYTES / 4);
+    const uint64_t pitch = (uint64_t)c.K / 2;
     rc = encode_tmap_3d(&maps.tok, BTM_U8, c.act, pitch, (uint64_t)c.rows, 1, pitch, pitch, 128, (uint32_t)a.box_rows);
     if (!rc) rc = encode_tmap_3d(&maps.w, BTM_U8, c.w, pitch, (uint64_t)c.N, (uint64_t)c.groups, pitch, pitch * (uint64_t)c.N, 128, BW);
-    if (!rc) rc = encode_tmap_3d(&maps.sft, BTM_U32, c.act_scales, words, (uint64_t)grouped_slot_bound(c.groups, c.rows), 1, words * 4, words * 4, 256, 1, 0);
-    if (!rc) rc = encode_tmap_3d(&maps.sfw, BTM_U32, c.w_scales, words, (uint64_t)a.n_blocks, (uint64_t)c.groups, words * 4, words * 4 * (uint64_t)a.n_blocks, 256, 1, 0);
+    if (!rc) rc = encode_mx_scales(&maps.sft, c.act_scales, c.K, (uint64_t)grouped_slot_bound(c.groups, c.rows), 1, 1);
+    if (!rc) rc = encode_mx_scales(&maps.sfw, c.w_scales, c.K, (uint64_t)a.n_blocks, (uint64_t)c.groups, 1);
     if (rc) return rc;
     return c.dtype == BTM_F16 ? launch_decode<BTM_F16, DECODE_MX>(st, maps, a, split, blocks) : launch_decode<BTM_BF16, DECODE_MX>(st, maps, a, split, blocks);
 }

@@ -116,6 +116,29 @@ __device__ __forceinline__ GroupedTile grouped_tile_uniform(const GemmParams &p,
     return o;
 }
 
+// The first n of eight 16-bit values to an address that is a multiple of two bytes: in pairs where it is one of four, else
+// one, three pairs and one.
+__device__ __forceinline__ void store8_unaligned(uint16_t *q, const uint4 &v, int n)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if ((reinterpret_cast<uintptr_t>(q) & 2) == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (2 * i + 1 < n) *reinterpret_cast<uint32_t *>(q + 2 * i) = w[i];
+            else if (2 * i < n) q[2 * i] = (uint16_t)w[i];
+        }
+    } else {
+        q[0] = (uint16_t)w[0];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const uint32_t pair = __funnelshift_r(w[i], w[i + 1], 16);
+            if (2 * i + 2 < n) *reinterpret_cast<uint32_t *>(q + 2 * i + 1) = pair;
+            else if (2 * i + 1 < n) q[2 * i + 1] = (uint16_t)pair;
+        }
+        if (n == 8) q[7] = (uint16_t)(w[3] >> 16);
+    }
+}
+
 // One 32-row band of a finished tile to C. `rows_end`: rows from here on are not this tile's. zero: the sum is empty.
 template <int DT, bool kWgrad>
 __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensorMap &tmC, uint32_t tmem_band, const GroupedTile &t, int row0,
@@ -157,24 +180,6 @@ __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensor
                 tma_store_3d(&tmC, buf, col, row0, z);
                 bulk_commit();
             }
-        } else if (!p.c_vec_ok) {
-            // Rows of C that start anywhere: two bytes per lane, a warp writes 64 contiguous bytes of a row.
-            __syncwarp();
-            uint16_t *dst = reinterpret_cast<uint16_t *>(p.C[0]);
-            const int rows = min(32, rows_end - row0), cols = min(64, p.N - col);
-#pragma unroll 4
-            for (int r = 0; r < rows; ++r) {
-                const long long off = base + (long long)(row0 + r) * p.ldc + col;
-                if (!store_in_bounds(p, off, cols)) continue;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int e = h * 32 + lane;
-                    uint16_t v;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(buf + (uint32_t)r * 128u + ((((uint32_t)(e >> 3)) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(e & 7) * 2u));
-                    if (e < cols) dst[off + e] = v;
-                }
-            }
-            if (lane == 0) bulk_commit();
         } else {
             __syncwarp();
             uint16_t *dst = reinterpret_cast<uint16_t *>(p.C[0]);
@@ -189,14 +194,8 @@ __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensor
                                  : "r"(buf + (uint32_t)r * 128u + (((uint32_t)(j ^ (r & 7))) << 4)));
                     const long long off = base + (long long)row * p.ldc + ccol;
                     if (store_in_bounds(p, off, min(8, p.N - ccol))) {
-                        if (ccol + 8 <= p.N) {
-                            *reinterpret_cast<uint4 *>(dst + off) = v;
-                        } else {
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (ccol + e < p.N) dst[off + e] = (uint16_t)((e & 1) ? (w[e >> 1] >> 16) : (w[e >> 1] & 0xFFFFu));
-                        }
+                        if (p.c_vec_ok && ccol + 8 <= p.N) *reinterpret_cast<uint4 *>(dst + off) = v;
+                        else store8_unaligned(dst + off, v, min(8, p.N - ccol));
                     }
                 }
             }

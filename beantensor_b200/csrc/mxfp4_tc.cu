@@ -3,10 +3,11 @@
 //
 // tcgen05.mma kind::mxf4.block_scale multiplies the 4-bit values and applies both scales; no value is ever unpacked. Both
 // operands are K-major as they lie (256 k = 128 bytes, 128-byte swizzle). The scales lie in memory in the order in which
-// tensor memory holds them: a block of 128 rows x 128 k comes in by an untiled bulk copy with its stage and goes to
-// tensor memory by one tcgen05.cp.
+// tensor memory holds them: as a matrix of 32-bit words, one block of 128 rows per row, they come in with their stage (two
+// blocks of the weights in one box) and go to tensor memory by one tcgen05.cp per 128 rows x 128 k.
 // One persistent CTA per SM, warp roles and tile walk as in gemm_grouped.cu (a plain product is one group that owns every
-// row).
+// row), and a second producer warp for the scales: issuing a TMA load takes a thread 75 to 120 cycles, a stage has four
+// to seven, and its MMAs take 384.
 #include <cstdlib>
 #include <cstring>
 
@@ -25,7 +26,6 @@ constexpr int BM = 128;               // token rows of a tile
 constexpr int BN = 192;               // widest tile: two accumulators of 192 columns leave tensor memory for the scales
 constexpr int BK = 256;               // k per stage: 128 bytes
 constexpr int A_BYTES = BM * 128;
-constexpr int CHUNK_BYTES = 64 * 128; // one box of weights: 64 rows
 constexpr int SFA_AT = A_BYTES + BN * 128;
 constexpr int SFB_AT = SFA_AT + 2 * MX_SCALE_BYTES;        // two row blocks, two k-chunks each
 constexpr int STAGE_BYTES = SFB_AT + 4 * MX_SCALE_BYTES;   // 43 KB
@@ -34,22 +34,19 @@ constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_SMEM_BYTES + 1024;
 constexpr int SF_COL = 2 * BN;        // first tensor-memory column of the scales
 constexpr int SF_STAGE_COLS = 32;     // per stage: A 2 x 4 columns, B 2 x 8
 constexpr int TMEM_COLS = 512;
-constexpr int THREADS = 192;
+constexpr int THREADS = 224;             // warp 0 operands, 1 MMA, 2-5 epilogue, 6 scales
 constexpr int A_BAND = 32;
 static_assert(SF_COL + STAGES * SF_STAGE_COLS <= TMEM_COLS, "accumulators and scales share tensor memory");
 static_assert(STAGE_BYTES % 1024 == 0, "stages start on swizzle atoms");
 } // namespace mxt
 
-struct MxOperands {
-    const uint8_t *act_scales, *w_scales;
-    const int *offsets;
-    int groups, rows;
+struct MxMaps {
+    CUtensorMap a, a_band, b[3] /* 192, 128 and 64 weight rows per box */, sfa, sfb, c;
 };
 
 template <int DT>
 __global__ void __launch_bounds__(mxt::THREADS, 1)
-mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA_band, const __grid_constant__ CUtensorMap tmB,
-                  const __grid_constant__ CUtensorMap tmC, const __grid_constant__ GemmParams p, const MxOperands op)
+mxfp4_gemm_kernel(const __grid_constant__ MxMaps maps, const __grid_constant__ GemmParams p, const GroupedTables tab)
 {
     using namespace mxt;
     extern __shared__ uint8_t smem_raw[];
@@ -70,9 +67,10 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             mbar_init(smem_u32(&bar_tmem_empty[a]), 4);
         }
         fence_mbar_init();
-        prefetch_tmap(&tmA);
-        prefetch_tmap(&tmA_band);
-        prefetch_tmap(&tmB);
+        prefetch_tmap(&maps.a);
+        prefetch_tmap(&maps.a_band);
+        prefetch_tmap(&maps.sfa);
+        prefetch_tmap(&maps.sfb);
     }
     if (warp == 1) {
         tmem_alloc<1>(smem_u32(&tmem_base_holder), TMEM_COLS);
@@ -86,43 +84,38 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     GroupWalk<> walk;
-    walk.init(op.offsets, op.groups, op.rows);
+    walk.init(tab.offsets, tab.groups, tab.rows);
     const GroupedPlan plan = plan_tiles<BN>(walk.count_slots(), p.N, gridDim.x);
     if (blockIdx.x == 0 && warp == 0) walk.report(p.status);
-    const int k_chunks = mx_chunks(p.K), n_blocks = (p.N + 127) / 128;
 
-    if (warp == 0) {
-        // ------------------------------------------------------------ TMA producer
+    if (warp == 0 || warp == 6) {
+        // ------------------------------------------------------------ TMA producers: operands, scales
         int stage = 0;
         uint32_t phase = 0;
         bool ok = !p.debug_skip_loads;
         for (int tile = blockIdx.x; ok && tile < plan.total; tile += gridDim.x) {
             const GroupedTile t = grouped_tile_uniform<false, GROUP_SLOT_ROWS>(p, plan, walk, tile);
             const int bands = min(4, (t.hi - t.m0 + A_BAND - 1) / A_BAND);
-            const int chunks = t.bn / 64;
-            const int nb0 = t.n0 / 128;
-            const int nb = min(n_blocks, (t.n0 + t.bn + 127) / 128) - nb0; // row blocks of weight scales: 1 or 2
-            const uint8_t *sfa = op.act_scales + (long long)t.slot * k_chunks * MX_SCALE_BYTES;
-            const uint8_t *sfb = op.w_scales + ((long long)t.g * n_blocks + nb0) * k_chunks * MX_SCALE_BYTES;
+            const uint32_t bytes = (uint32_t)(bands * A_BAND * 128 + t.bn * 128 + 6 * MX_SCALE_BYTES);
+            const CUtensorMap *mb = &maps.b[t.bn == BN ? 0 : t.bn == 128 ? 1 : 2];
             for (int kb = 0; kb < p.num_kb; ++kb) {
                 ok = mbar_wait_uniform(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag, p.status, WAIT_PRODUCER_EMPTY, p.wait_limit);
                 if (!ok) break;
                 if (elect_one()) {
                     const uint32_t full = smem_u32(&bar_full[stage]);
-                    const uint32_t a0 = smem_base + stage * STAGE_BYTES, b0 = a0 + A_BYTES;
-                    const uint32_t sf_bytes = (uint32_t)min(2, k_chunks - kb * 2) * MX_SCALE_BYTES;
-                    mbar_expect_tx(full, (uint32_t)(bands * A_BAND * 128 + chunks * CHUNK_BYTES) + sf_bytes * (uint32_t)(1 + nb));
-                    if (bands == 4) {
-                        tma_load_3d(a0, &tmA, kb * 128, t.m0, 0, full);
+                    const uint32_t a0 = smem_base + stage * STAGE_BYTES;
+                    if (warp == 0) {
+                        mbar_expect_tx(full, bytes);
+                        if (bands == 4) {
+                            tma_load_3d(a0, &maps.a, kb * 128, t.m0, 0, full);
+                        } else {
+                            for (int b = 0; b < bands; ++b) tma_load_3d(a0 + b * A_BAND * 128, &maps.a_band, kb * 128, t.m0 + b * A_BAND, 0, full);
+                        }
+                        tma_load_3d(a0 + A_BYTES, mb, kb * 128, t.n0, t.g, full);
                     } else {
-                        for (int b = 0; b < bands; ++b) tma_load_3d(a0 + b * A_BAND * 128, &tmA_band, kb * 128, t.m0 + b * A_BAND, 0, full);
+                        tma_load_3d(a0 + SFA_AT, &maps.sfa, kb * 256, t.slot, 0, full);
+                        tma_load_3d(a0 + SFB_AT, &maps.sfb, kb * 256, t.n0 / 128, t.g, full);
                     }
-#pragma unroll
-                    for (int c = 0; c < BN / 64; ++c)
-                        if (c < chunks) tma_load_3d(b0 + c * CHUNK_BYTES, &tmB, kb * 128, t.n0 + c * 64, t.g, full);
-                    bulk_load(a0 + SFA_AT, sfa + kb * 2 * MX_SCALE_BYTES, sf_bytes, full);
-                    for (int b = 0; b < nb; ++b)
-                        bulk_load(a0 + SFB_AT + b * 2 * MX_SCALE_BYTES, sfb + ((long long)b * k_chunks + kb * 2) * MX_SCALE_BYTES, sf_bytes, full);
                 }
                 __syncwarp();
                 if (++stage == STAGES) {
@@ -191,7 +184,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             const int acc = it & 1;
             if (!mbar_wait_uniform(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();
-            grouped_band<DT, false>(p, tmC, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t, t.m0 + quad * 32, t.hi, false,
+            grouped_band<DT, false>(p, maps.c, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t, t.m0 + quad * 32, t.hi, false,
                                     epi_smem, epi_tiles, lane);
             tc_fence_before();
             __syncwarp();
@@ -213,6 +206,13 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         tc_fence_after();
         tmem_dealloc<1>(tmem_base, TMEM_COLS);
     }
+}
+
+// Scale blocks as a matrix of 32-bit words, one row block per row: boxes of two k-chunks x `box_rows` row blocks.
+int encode_mx_scales(CUtensorMap *m, const void *scales, int K, uint64_t blocks, uint64_t groups, uint32_t box_rows)
+{
+    const uint64_t words = (uint64_t)mx_chunks(K) * (MX_SCALE_BYTES / 4);
+    return encode_tmap_3d(m, BTM_U32, scales, words, blocks, groups, words * 4, words * 4 * blocks, 2 * MX_SCALE_BYTES / 4, box_rows, 0);
 }
 
 int configure_mxfp4_kernels()
@@ -239,11 +239,12 @@ int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
     const long long most = slots * ((c.N + 63) / 64);
     if (most > 0x3FFFFFFFLL) return set_error(BTM_ERR_UNSUPPORTED, "mxfp4 matmul: too many output tiles (%lld)", most);
     const uint64_t pitch = (uint64_t)c.K / 2;
-    CUtensorMap tmA, tmA_band, tmB, tmC;
-    memset(&tmC, 0, sizeof(tmC));
-    int rc = encode_tmap_3d(&tmA, BTM_U8, c.act, pitch, (uint64_t)c.rows, 1, pitch, pitch, 128, BM);
-    if (!rc) rc = encode_tmap_3d(&tmA_band, BTM_U8, c.act, pitch, (uint64_t)c.rows, 1, pitch, pitch, 128, A_BAND);
-    if (!rc) rc = encode_tmap_3d(&tmB, BTM_U8, c.w, pitch, (uint64_t)c.N, (uint64_t)c.groups, pitch, pitch * (uint64_t)c.N, 128, 64);
+    MxMaps maps;
+    memset(&maps, 0, sizeof(maps));
+    int rc = encode_tmap_3d(&maps.a, BTM_U8, c.act, pitch, (uint64_t)c.rows, 1, pitch, pitch, 128, BM);
+    if (!rc) rc = encode_tmap_3d(&maps.a_band, BTM_U8, c.act, pitch, (uint64_t)c.rows, 1, pitch, pitch, 128, A_BAND);
+    if (!rc) rc = encode_mx_scales(&maps.sfa, c.act_scales, c.K, (uint64_t)slots, 1, 1);
+    if (!rc) rc = encode_mx_scales(&maps.sfb, c.w_scales, c.K, (uint64_t)((c.N + 127) / 128), (uint64_t)c.groups, 2);
     if (rc) return rc;
     GemmParams p;
     memset(&p, 0, sizeof(p));
@@ -260,7 +261,7 @@ int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
     p.status = status;
     fill_wait_params(&p);
     if (p.c_vec_ok) {
-        rc = encode_tmap_3d(&tmC, c.dtype, c.out, (uint64_t)c.N, (uint64_t)c.rows, 1, (uint64_t)c.ldo * 2, (uint64_t)c.ldo * 2, 64, 32);
+        rc = encode_tmap_3d(&maps.c, c.dtype, c.out, (uint64_t)c.N, (uint64_t)c.rows, 1, (uint64_t)c.ldo * 2, (uint64_t)c.ldo * 2, 64, 32);
         if (rc) return rc;
     }
     // Pairs of CTAs for tall groups and a reduction that pays for their set-up. Measured, one CTA against pairs, rows / N x K:
@@ -271,8 +272,11 @@ int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
         if (!strcmp(force, "1cta")) pair = false;
         else if (!strcmp(force, "2cta")) pair = true;
     }
-    if (pair) return launch_mxfp4_matmul_pair(c, st, sm_count, p, tmA, tmA_band, tmC);
-    const MxOperands op = {(const uint8_t *)c.act_scales, (const uint8_t *)c.w_scales, c.offsets, c.groups, c.rows};
+    if (pair) return launch_mxfp4_matmul_pair(c, st, sm_count, p, maps.a, maps.a_band, maps.sfa, maps.sfb, maps.c);
+    static const uint32_t box_rows[3] = {BN, 128, 64};
+    for (int i = 0; i < 3 && !rc; ++i) rc = encode_tmap_3d(&maps.b[i], BTM_U8, c.w, pitch, (uint64_t)c.N, (uint64_t)c.groups, pitch, pitch * (uint64_t)c.N, 128, box_rows[i]);
+    if (rc) return rc;
+    const GroupedTables tab = {c.offsets, c.groups, c.rows};
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)(most < sm_count ? most : sm_count), 1, 1);
@@ -284,8 +288,8 @@ int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = c.dtype == BTM_F16 ? cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<BTM_F16>, tmA, tmA_band, tmB, tmC, p, op)
-                                             : cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<BTM_BF16>, tmA, tmA_band, tmB, tmC, p, op);
+    const cudaError_t e = c.dtype == BTM_F16 ? cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<BTM_F16>, maps, p, tab)
+                                             : cudaLaunchKernelEx(&cfg, mxfp4_gemm_kernel<BTM_BF16>, maps, p, tab);
     return check_cuda(e, "mxfp4 matmul launch");
 }
 

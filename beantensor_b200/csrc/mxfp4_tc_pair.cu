@@ -224,15 +224,8 @@ mxfp4_gemm_pair_kernel(const __grid_constant__ MxPairMaps maps, const __grid_con
     }
 }
 
-// Scale blocks as a matrix of 32-bit words, one row block per row: boxes of two k-chunks x `box_rows` row blocks.
-static int encode_scales(CUtensorMap *m, const void *scales, int K, uint64_t blocks, uint64_t groups, uint32_t box_rows)
-{
-    const uint64_t words = (uint64_t)mx_chunks(K) * (MX_SCALE_BYTES / 4);
-    return encode_tmap_3d(m, BTM_U32, scales, words, blocks, groups, words * 4, words * 4 * blocks, 2 * MX_SCALE_BYTES / 4, box_rows, 0);
-}
-
 int launch_mxfp4_matmul_pair(const Mxfp4Call &c, cudaStream_t st, int sm_count, const GemmParams &p, const CUtensorMap &tmA, const CUtensorMap &tmA_band,
-                             const CUtensorMap &tmC)
+                             const CUtensorMap &sfa, const CUtensorMap &sfb, const CUtensorMap &tmC)
 {
     using namespace mxp;
     const uint64_t pitch = (uint64_t)c.K / 2;
@@ -240,11 +233,11 @@ int launch_mxfp4_matmul_pair(const Mxfp4Call &c, cudaStream_t st, int sm_count, 
     memset(&maps, 0, sizeof(maps));
     maps.a = tmA;
     maps.a_band = tmA_band;
+    maps.sfa = sfa;
+    maps.sfb = sfb;
     maps.c = tmC;
     int rc = encode_tmap_3d(&maps.b_wide, BTM_U8, c.w, pitch, (uint64_t)c.N, (uint64_t)c.groups, pitch, pitch * (uint64_t)c.N, 128, BN / 2);
     if (!rc) rc = encode_tmap_3d(&maps.b_narrow, BTM_U8, c.w, pitch, (uint64_t)c.N, (uint64_t)c.groups, pitch, pitch * (uint64_t)c.N, 128, 64);
-    if (!rc) rc = encode_scales(&maps.sfa, c.act_scales, c.K, (uint64_t)grouped_slot_bound(c.groups, c.rows), 1, 1);
-    if (!rc) rc = encode_scales(&maps.sfb, c.w_scales, c.K, (uint64_t)((c.N + 127) / 128), (uint64_t)c.groups, 2);
     if (rc) return rc;
     static std::atomic<int> resident[64]; // pairs the device holds at once (GPC boundaries can make it less than SMs / 2)
     int dev = 0;
