@@ -4,7 +4,7 @@
 //   weight gradient:  C[g]    = A[rows of g]^T . D[rows of g]    (all zero for a group without rows)
 //
 // Tensor-core kernel: one persistent CTA per SM with the warp roles of gemm_tc.cu (TMA producer, tcgen05.mma issuer with
-// two accumulators in tensor memory, four epilogue warps). What differs is where a tile's rows come from: every role
+// two accumulators in tensor memory, eight epilogue warps). What differs is where a tile's rows come from: every role
 // walks the table by itself, a warp at a time, and no tile list exists in memory.
 //   product    rows are cut per group into slots of 128; a tile is (slot, column range). A tile reads up to 128 rows of
 //              A from the group's first row on, whatever alignment that has (a row coordinate is free), so rows of the
@@ -45,7 +45,7 @@ constexpr int RING_BYTES = 4 * (A_BYTES + BN * 128);
 constexpr int STAGES = 8;
 constexpr int SMEM_BYTES = RING_BYTES + EPI_SMEM_BYTES + 1024;
 constexpr int TMEM_COLS = 512;
-constexpr int THREADS = 192;
+constexpr int THREADS = 320; // warp 0 TMA, 1 MMA, 2-9 epilogue;
 constexpr int A_BAND = 32;              // rows of a short A box: a tile with few rows does not fetch its neighbours'
 } // namespace gg
 
@@ -73,7 +73,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(smem_u32(&bar_tmem_full[a]), 1);
-            mbar_init(smem_u32(&bar_tmem_empty[a]), 4);
+            mbar_init(smem_u32(&bar_tmem_empty[a]), GROUPED_EPI_WARPS);
         }
         fence_mbar_init();
         prefetch_tmap(&tmA);
@@ -203,10 +203,9 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             __syncwarp();
         }
     } else {
-        // ------------------------------------------------------------ epilogue (warps 2..5)
+        // ------------------------------------------------------------ epilogue (warps 2..9)
         const int quad = warp & 3;
-        const uint32_t epi_smem = smem_base + RING_BYTES + (uint32_t)quad * EPI_WARP_BYTES;
-        uint32_t epi_tiles = 0;
+        const uint32_t epi_smem = smem_base + RING_BYTES + (uint32_t)(warp - 2) * EPI_TILE_BYTES;
         int it = 0;
         for (int tile = blockIdx.x; tile < plan.total; tile += gridDim.x, ++it) {
             const GroupedTile t = grouped_tile<kWgrad, GROUP_SLOT_ROWS>(p, plan, walk, tile);
@@ -214,7 +213,7 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             if (!mbar_wait_uniform(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();
             grouped_band<DT, kWgrad>(p, tmC, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t, t.m0 + quad * 32,
-                                   kWgrad ? p.M : t.hi, kWgrad && t.lo == t.hi, epi_smem, epi_tiles, lane);
+                                   kWgrad ? p.M : t.hi, kWgrad && t.lo == t.hi, epi_smem, (warp - 2) >> 2, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));

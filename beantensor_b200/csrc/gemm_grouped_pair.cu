@@ -3,7 +3,7 @@
 // k-block costs it 32 KB instead of 48 KB and the ring holds half as many k-blocks again: what bounds the one-CTA form with many
 // rows is the latency of its loads, since the matrices of different groups come from HBM one after the other. Barriers
 // as in gemm_tc2.cu: full[s] lives in the leader and counts the bytes of both CTAs; empty[s] and tmem_full[a] are signalled in
-// both by multicast tcgen05.commit; tmem_empty[a] lives in the leader and collects the eight epilogue warps. No TMA
+// both by multicast tcgen05.commit; tmem_empty[a] lives in the leader and collects the sixteen epilogue warps. No TMA
 // multicast is used.
 //
 // Rows of a group are cut into slots of 256; in a group's last slot the second CTA may own no row: it then loads none of
@@ -35,7 +35,7 @@ constexpr int STAGE_BYTES = KPS * KB_BYTES;
 constexpr int STAGES = 3;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_SMEM_BYTES + 1024;
 constexpr int TMEM_COLS = 512;
-constexpr int THREADS = 192;
+constexpr int THREADS = 320; // warp 0 TMA, 1 MMA, 2-9 epilogue;
 constexpr int A_BAND = 32;
 } // namespace gp
 
@@ -66,7 +66,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(smem_u32(&bar_tmem_full[a]), 1);
-            mbar_init(smem_u32(&bar_tmem_empty[a]), 8);
+            mbar_init(smem_u32(&bar_tmem_empty[a]), 2 * GROUPED_EPI_WARPS);
         }
         fence_mbar_init();
         prefetch_tmap(&tmA);
@@ -186,8 +186,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
     } else if (warp >= 2) {
         // ------------------------------------------------------------ epilogue (both CTAs, own 128 rows)
         const int quad = warp & 3;
-        const uint32_t epi_smem = smem_base + STAGES * STAGE_BYTES + (uint32_t)quad * EPI_WARP_BYTES;
-        uint32_t epi_tiles = 0;
+        const uint32_t epi_smem = smem_base + STAGES * STAGE_BYTES + (uint32_t)(warp - 2) * EPI_TILE_BYTES;
         int it = 0;
         for (int tile = pair_id; tile < plan.total; tile += num_pairs, ++it) {
             const GroupedTile t = grouped_tile<false, PAIR_M>(p, plan, walk, tile);
@@ -195,7 +194,7 @@ gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_c
             if (!mbar_wait_uniform<true>(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();
             grouped_band<DT, false>(p, tmC, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t,
-                                     t.m0 + (int)rank * CTA_M + quad * 32, t.hi, false, epi_smem, epi_tiles, lane);
+                                     t.m0 + (int)rank * CTA_M + quad * 32, t.hi, false, epi_smem, (warp - 2) >> 2, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {

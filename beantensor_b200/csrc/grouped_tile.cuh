@@ -139,10 +139,17 @@ __device__ __forceinline__ void store8_unaligned(uint16_t *q, const uint4 &v, in
     }
 }
 
-// One 32-row band of a finished tile to C. `rows_end`: rows from here on are not this tile's. zero: the sum is empty.
+// Eight epilogue warps, two per tensor-memory quadrant: they take alternate 64-column chunks of a band, each with a staging
+// tile of its own. (One per quadrant with two tiles drained a 128 x 256 tile in about 2600 cycles, more than the main
+// loop of a shallow product takes.)
+constexpr int GROUPED_EPI_WARPS = 8;
+static_assert(GROUPED_EPI_WARPS * EPI_TILE_BYTES == EPI_SMEM_BYTES, "one staging tile per epilogue warp");
+
+// One 32-row band of a finished tile to C, the chunks first_chunk, first_chunk + 2, .. of it. `rows_end`: rows from here on are
+// not this tile's. zero: the sum is empty.
 template <int DT, bool kWgrad>
 __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensorMap &tmC, uint32_t tmem_band, const GroupedTile &t, int row0,
-                                             int rows_end, bool zero, uint32_t epi_smem, uint32_t &tile_count, int lane)
+                                             int rows_end, bool zero, uint32_t buf, int first_chunk, int lane)
 {
     if (row0 >= rows_end) return;
     const int z = kWgrad ? t.g : 0;
@@ -150,15 +157,13 @@ __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensor
     const uint32_t swz = (uint32_t)(lane & 7);
     const bool whole = p.c_vec_ok && (kWgrad || row0 + 32 <= rows_end); // C[g] is clipped by its tensor map
 #pragma unroll 1
-    for (int c = 0; c < t.bn / 64; ++c) {
+    for (int c = first_chunk; c < t.bn / 64; c += 2) {
         const int col = t.n0 + c * 64;
         if (col >= p.N) break;
-        const uint32_t buf = epi_smem + (tile_count & 1u) * EPI_TILE_BYTES;
-        ++tile_count;
         uint32_t v0[32], v1[32];
         tmem_ld_32x32(tmem_band + (uint32_t)(c * 64), v0);
         tmem_ld_32x32(tmem_band + (uint32_t)(c * 64 + 32), v1);
-        if (lane == 0) bulk_wait_read<1>(); // the store of two chunks ago has read this buffer
+        if (lane == 0) bulk_wait_read<0>(); // the store before has read the staging tile
         __syncwarp();
         tmem_ld_wait();
 #pragma unroll
@@ -199,7 +204,6 @@ __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensor
                     }
                 }
             }
-            if (lane == 0) bulk_commit(); // an empty group keeps the buffer accounting uniform
         }
     }
 }

@@ -34,7 +34,7 @@ constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_SMEM_BYTES + 1024;
 constexpr int SF_COL = 2 * BN;        // first tensor-memory column of the scales
 constexpr int SF_STAGE_COLS = 32;     // per stage: A 2 x 4 columns, B 2 x 8
 constexpr int TMEM_COLS = 512;
-constexpr int THREADS = 224;             // warp 0 operands, 1 MMA, 2-5 epilogue, 6 scales
+constexpr int THREADS = 352; // warp 0 operands, 1 MMA, 2-9 epilogue, 10 scales;
 constexpr int A_BAND = 32;
 static_assert(SF_COL + STAGES * SF_STAGE_COLS <= TMEM_COLS, "accumulators and scales share tensor memory");
 static_assert(STAGE_BYTES % 1024 == 0, "stages start on swizzle atoms");
@@ -64,7 +64,7 @@ mxfp4_gemm_kernel(const __grid_constant__ MxMaps maps, const __grid_constant__ G
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(smem_u32(&bar_tmem_full[a]), 1);
-            mbar_init(smem_u32(&bar_tmem_empty[a]), 4);
+            mbar_init(smem_u32(&bar_tmem_empty[a]), GROUPED_EPI_WARPS);
         }
         fence_mbar_init();
         prefetch_tmap(&maps.a);
@@ -88,7 +88,7 @@ mxfp4_gemm_kernel(const __grid_constant__ MxMaps maps, const __grid_constant__ G
     const GroupedPlan plan = plan_tiles<BN>(walk.count_slots(), p.N, gridDim.x);
     if (blockIdx.x == 0 && warp == 0) walk.report(p.status);
 
-    if (warp == 0 || warp == 6) {
+    if (warp == 0 || warp == 10) {
         // ------------------------------------------------------------ TMA producers: operands, scales
         int stage = 0;
         uint32_t phase = 0;
@@ -174,10 +174,9 @@ mxfp4_gemm_kernel(const __grid_constant__ MxMaps maps, const __grid_constant__ G
             __syncwarp();
         }
     } else {
-        // ------------------------------------------------------------ epilogue (warps 2..5)
+        // ------------------------------------------------------------ epilogue (warps 2..9)
         const int quad = warp & 3;
-        const uint32_t epi_smem = smem_base + STAGES * STAGE_BYTES + (uint32_t)quad * EPI_WARP_BYTES;
-        uint32_t epi_tiles = 0;
+        const uint32_t epi_smem = smem_base + STAGES * STAGE_BYTES + (uint32_t)(warp - 2) * EPI_TILE_BYTES;
         int it = 0;
         for (int tile = blockIdx.x; tile < plan.total; tile += gridDim.x, ++it) {
             const GroupedTile t = grouped_tile<false, GROUP_SLOT_ROWS>(p, plan, walk, tile);
@@ -185,7 +184,7 @@ mxfp4_gemm_kernel(const __grid_constant__ MxMaps maps, const __grid_constant__ G
             if (!mbar_wait_uniform(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();
             grouped_band<DT, false>(p, maps.c, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t, t.m0 + quad * 32, t.hi, false,
-                                    epi_smem, epi_tiles, lane);
+                                    epi_smem, (warp - 2) >> 2, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));

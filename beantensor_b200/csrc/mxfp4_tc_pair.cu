@@ -34,7 +34,7 @@ constexpr int SF_STAGE_COLS = 24; // A 2 x 4 columns, B 2 x 8
 constexpr int STAGES = 5;         // as many as there are columns for their scales
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_SMEM_BYTES + 1024;
 constexpr int TMEM_COLS = 512;
-constexpr int THREADS = 224; // warp 0 operands, 1 MMA, 2-5 epilogue, 6 scales
+constexpr int THREADS = 352; // warp 0 operands, 1 MMA, 2-9 epilogue, 10 scales;
 constexpr int A_BAND = 32;
 static_assert(SF_COL + STAGES * SF_STAGE_COLS <= TMEM_COLS, "accumulators and scales share tensor memory");
 static_assert(STAGE_BYTES % 1024 == 0, "stages start on swizzle atoms");
@@ -69,7 +69,7 @@ mxfp4_gemm_pair_kernel(const __grid_constant__ MxPairMaps maps, const __grid_con
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(smem_u32(&bar_tmem_full[a]), 1);
-            mbar_init(smem_u32(&bar_tmem_empty[a]), 8);
+            mbar_init(smem_u32(&bar_tmem_empty[a]), 2 * GROUPED_EPI_WARPS);
         }
         fence_mbar_init();
         prefetch_tmap(&maps.a);
@@ -96,7 +96,7 @@ mxfp4_gemm_pair_kernel(const __grid_constant__ MxPairMaps maps, const __grid_con
     const GroupedPlan plan = plan_tiles<BN, 128>(walk.count_slots(), p.N, num_pairs);
     if (blockIdx.x == 0 && warp == 0) walk.report(p.status);
 
-    if (warp == 0 || warp == 6) {
+    if (warp == 0 || warp == 10) {
         // ------------------------------------------------------------ TMA producers (both CTAs): operands, scales
         int stage = 0;
         uint32_t phase = 0;
@@ -185,10 +185,9 @@ mxfp4_gemm_pair_kernel(const __grid_constant__ MxPairMaps maps, const __grid_con
             __syncwarp();
         }
     } else if (warp >= 2) {
-        // ------------------------------------------------------------ epilogue (warps 2..5 of both CTAs, own 128 rows)
+        // ------------------------------------------------------------ epilogue (warps 2..9 of both CTAs, own 128 rows)
         const int quad = warp & 3;
-        const uint32_t epi_smem = smem_base + STAGES * STAGE_BYTES + (uint32_t)quad * EPI_WARP_BYTES;
-        uint32_t epi_tiles = 0;
+        const uint32_t epi_smem = smem_base + STAGES * STAGE_BYTES + (uint32_t)(warp - 2) * EPI_TILE_BYTES;
         int it = 0;
         for (int tile = pair_id; tile < plan.total; tile += num_pairs, ++it) {
             const GroupedTile t = grouped_tile<false, PAIR_M>(p, plan, walk, tile);
@@ -196,7 +195,7 @@ mxfp4_gemm_pair_kernel(const __grid_constant__ MxPairMaps maps, const __grid_con
             if (!mbar_wait_uniform<true>(smem_u32(&bar_tmem_full[acc]), (uint32_t)(it >> 1) & 1u, &abort_flag, p.status, WAIT_EPI_TMEM_FULL, p.wait_limit)) break;
             tc_fence_after();
             grouped_band<DT, false>(p, maps.c, tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN), t,
-                                    t.m0 + (int)rank * CTA_M + quad * 32, t.hi, false, epi_smem, epi_tiles, lane);
+                                    t.m0 + (int)rank * CTA_M + quad * 32, t.hi, false, epi_smem, (warp - 2) >> 2, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
