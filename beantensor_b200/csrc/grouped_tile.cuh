@@ -116,26 +116,44 @@ __device__ __forceinline__ GroupedTile grouped_tile_uniform(const GemmParams &p,
     return o;
 }
 
-// The first n of eight 16-bit values to an address that is a multiple of two bytes: in pairs where it is one of four, else
-// one, three pairs and one.
-__device__ __forceinline__ void store8_unaligned(uint16_t *q, const uint4 &v, int n)
+// Rows of 64 values from a staging tile to rows of C that start anywhere (multiples of two bytes). Lane l holds the values
+// 2 l and 2 l + 1 of a row: where the row starts on four bytes it stores them as they are, where it starts between, the pair
+// 2 l - 1, 2 l with its neighbour's second value, and the ends alone. So a warp instruction writes one row's 128 contiguous
+// bytes; 16-byte pieces stored in parts would touch every sector four or five times, and the store path takes about a
+// sector per cycle.
+__device__ __forceinline__ void store_rows_unaligned(uint32_t buf, uint16_t *c, long long ldc, int rows, int cols, int lane)
 {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    if ((reinterpret_cast<uintptr_t>(q) & 2) == 0) {
+    uint16_t *q = c + 2 * lane;
+    if (cols == 64) {
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+            uint32_t w[8], pair[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (2 * i + 1 < n) *reinterpret_cast<uint32_t *>(q + 2 * i) = w[i];
-            else if (2 * i < n) q[2 * i] = (uint16_t)w[i];
-        }
-    } else {
-        q[0] = (uint16_t)w[0];
+            for (int i = 0; i < 8; ++i)
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(buf + (uint32_t)(r0 + i) * 128u + ((((uint32_t)lane >> 2) ^ (uint32_t)i) << 4) + (uint32_t)(lane & 3) * 4u));
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const uint32_t pair = __funnelshift_r(w[i], w[i + 1], 16);
-            if (2 * i + 2 < n) *reinterpret_cast<uint32_t *>(q + 2 * i + 1) = pair;
-            else if (2 * i + 1 < n) q[2 * i + 1] = (uint16_t)pair;
+            for (int i = 0; i < 8; ++i) pair[i] = __funnelshift_r(__shfl_up_sync(0xffffffffu, w[i], 1), w[i], 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (r0 + i < rows) {
+                    if ((reinterpret_cast<uintptr_t>(q) & 2) == 0) { // the same in all lanes
+                        *reinterpret_cast<uint32_t *>(q) = w[i];
+                    } else {
+                        if (lane > 0) *reinterpret_cast<uint32_t *>(q - 1) = pair[i];
+                        else *q = (uint16_t)w[i];
+                        if (lane == 31) q[1] = (uint16_t)(w[i] >> 16);
+                    }
+                }
+                q += ldc;
+            }
         }
-        if (n == 8) q[7] = (uint16_t)(w[3] >> 16);
+        return;
+    }
+    for (int r = 0; r < rows; ++r, q += ldc) { // the last columns of the matrix
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(buf + (uint32_t)r * 128u + ((((uint32_t)lane >> 2) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(lane & 3) * 4u));
+        if (2 * lane < cols) q[0] = (uint16_t)w;
+        if (2 * lane + 1 < cols) q[1] = (uint16_t)(w >> 16);
     }
 }
 
@@ -185,24 +203,31 @@ __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensor
                 tma_store_3d(&tmC, buf, col, row0, z);
                 bulk_commit();
             }
+        } else if (!p.c_vec_ok || col + 64 > p.N) {
+            __syncwarp();
+            const int cols = min(64, p.N - col);
+            const long long off = base + (long long)row0 * p.ldc + col;
+            int rows = min(32, rows_end - row0);
+            while (p.debug_bounds && rows > 0 && !store_in_bounds(p, off + (long long)(rows - 1) * p.ldc, cols)) --rows;
+            store_rows_unaligned(buf, reinterpret_cast<uint16_t *>(p.C[0]) + off, p.ldc, rows, cols, lane);
         } else {
+            // The group ends inside the band: 16-byte pieces of its own rows, all of a lane's in flight.
             __syncwarp();
             uint16_t *dst = reinterpret_cast<uint16_t *>(p.C[0]);
-            const int j = lane & 7, ccol = col + j * 8;
+            const int j = lane & 7, r_first = lane >> 3;
+            uint4 v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + (lane >> 3), row = row0 + r;
-                if (row < rows_end && ccol < p.N) {
-                    uint4 v;
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                 : "r"(buf + (uint32_t)r * 128u + (((uint32_t)(j ^ (r & 7))) << 4)));
-                    const long long off = base + (long long)row * p.ldc + ccol;
-                    if (store_in_bounds(p, off, min(8, p.N - ccol))) {
-                        if (p.c_vec_ok && ccol + 8 <= p.N) *reinterpret_cast<uint4 *>(dst + off) = v;
-                        else store8_unaligned(dst + off, v, min(8, p.N - ccol));
-                    }
-                }
+                const int r = i * 4 + r_first;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w)
+                             : "r"(buf + (uint32_t)r * 128u + (((uint32_t)(j ^ (r & 7))) << 4)));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = row0 + i * 4 + r_first;
+                const long long off = base + (long long)row * p.ldc + col + j * 8;
+                if (row < rows_end && store_in_bounds(p, off, 8)) *reinterpret_cast<uint4 *>(dst + off) = v[i];
             }
         }
     }
