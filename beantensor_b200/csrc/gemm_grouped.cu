@@ -473,10 +473,12 @@ int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int
         if (rc) return rc;
     }
     // Pairs of CTAs for tall and deep groups. Measured, one CTA against pairs, bf16, rows / N x K:
-    //   16384 in 8 groups, 4096 x 4096: 482 / 429 us       16384 in 16, 2048 x 4096: 266 / 241      12000 in 4, 2560 x 2560: 126 / 118
-    //   8192 in 8, 1024 x 1024: 23.1 / 22.3                16384 in 64, 2048 x 2048: 158 / 172      4096 in 16, 1024 x 512: 11.6 / 13.3
-    // so from 512 rows per group and K = 1024 on, with half as many tiles as there are pairs. The weight gradient has no pair form (gemm_grouped_pair.cu).
-    bool pair = !c.wgrad && c.rows / c.groups >= 512 && c.K >= 1024 && (long long)(c.rows / 256) * ((c.N + 255) / 256) >= sm_count / 4;
+    //   16384 in 8 groups / 4096 x 4096: 416 / 408 us    16384 in 16 / 2048 x 4096: 242 / 236    12000 in 4 / 2560 x 2560: 127 / 116
+    //   4096 in 16 / 2048 x 4096: 95.3 / 84.6    8192 in 8 / 1024 x 1024: 23.1 / 22.6    16384 in 64 / 2048 x 2048: 159 / 167
+    //   12000 in 64 / 1024 x 1024: 48.1 / 48.8
+    // The weight gradient has no pair form (gemm_grouped_pair.cu).
+    const long long height = c.rows / c.groups;
+    bool pair = !c.wgrad && height >= 256 && height * c.K > 512 * 1024 && (long long)(c.rows / 256) * ((c.N + 255) / 256) >= sm_count / 4;
     if (force) {
         if (!strcmp(force, "1cta")) pair = false;
         else if (!strcmp(force, "2cta")) pair = !c.wgrad;

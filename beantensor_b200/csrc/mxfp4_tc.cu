@@ -263,10 +263,10 @@ int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
         rc = encode_tmap_3d(&maps.c, c.dtype, c.out, (uint64_t)c.N, (uint64_t)c.rows, 1, (uint64_t)c.ldo * 2, (uint64_t)c.ldo * 2, 64, 32);
         if (rc) return rc;
     }
-    // Pairs of CTAs for tall groups and a reduction that pays for their set-up. Measured, one CTA against pairs, rows / N x K:
-    //   8192 / 11008 x 4096: 193 / 154 us    4096 / 4096 x 4096: 46.1 / 36.6    256 / 11008 x 4096: 11.9 / 10.4
-    //   16384 in 64 groups / 2048 x 2048: 63.2 / 60.5    8192 / 2048 x 1024: 17.2 / 17.9    3001 in 24 / 1000 x 1440: 15.9 / 17.4
-    bool pair = c.rows / c.groups >= 256 && c.K >= 1536;
+    // Pairs of CTAs for tall groups, a deep reduction and enough outputs for their larger tiles. Measured, one CTA against pairs,
+    // rows / N x K:  8192 / 11008 x 4096: 165 / 159 us    2048 / 4096 x 4096: 23.7 / 21.2    4096 in 8 groups / 4096 x 4096: 43.7 / 42.0
+    //   1024 / 4096 x 4096: 13.8 / 15.5    8192 / 2048 x 1024: 14.6 / 17.7    12000 in 24 groups / 4096 x 2048: 65.9 / 67.4
+    bool pair = c.rows / c.groups >= 512 && c.K >= 2048 && (long long)c.rows * c.N >= 8 << 20;
     if (force) {
         if (!strcmp(force, "1cta")) pair = false;
         else if (!strcmp(force, "2cta")) pair = true;
