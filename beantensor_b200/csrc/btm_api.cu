@@ -132,6 +132,8 @@ DeviceState *device_state(int device)
     if (configure_mxfp4_kernels()) return nullptr;
     if (configure_mxfp4_pair_kernels()) return nullptr;
     if (configure_grouped_decode_kernels()) return nullptr;
+    // Kernels without an attribute to set are looked up all the same, so that none is loaded in the middle of a capture.
+    if (load_grouped_simt_kernels() || load_mxfp4_convert_kernels()) return nullptr;
     if (configure_int4_gemv_kernels()) return nullptr;
     ds->sm_count = prop.multiProcessorCount;
     ds->ready.store(true, std::memory_order_release);
@@ -740,11 +742,19 @@ int btm_int4_quantize(int device, void *stream, int N, int K, int group, const v
     return launch_int4_quantize((cudaStream_t)stream, N, K, group, w_f16, out_packed, out_scales_f16);
 }
 
+// The grouped kernels round dimensions up to whole tiles in 32 bits, and every CTA walks the table of groups.
+static const int kMaxDim = 0x7FFFFFFF - 1024, kMaxGroups = 1 << 20;
+static int check_dims(const char *what, int a, int b, int c)
+{
+    if (a > kMaxDim || b > kMaxDim || c > kMaxDim) return set_error(BTM_ERR_UNSUPPORTED, "%s: dimensions (%d, %d, %d) above %d are not supported", what, a, b, c, kMaxDim);
+    return BTM_OK;
+}
 // Checks that the grouped operators share.
 static int check_groups(const char *what, int groups, int rows, const int32_t *offsets)
 {
     if (groups < 0 || rows < 0) return set_error(BTM_ERR_INVALID, "%s: negative dimension (groups=%d rows=%d)", what, groups, rows);
     if (groups > 0 && !offsets) return set_error(BTM_ERR_INVALID, "%s: null offsets", what);
+    if (groups > kMaxGroups) return set_error(BTM_ERR_UNSUPPORTED, "%s: %d groups are more than the %d that are supported", what, groups, kMaxGroups);
     if ((uintptr_t)offsets & 3) return set_error(BTM_ERR_INVALID, "%s: offsets are not aligned", what);
     return BTM_OK;
 }
@@ -756,6 +766,7 @@ int btm_gemm_grouped(int device, void *stream, int dtype, int groups, int rows, 
         return set_error(BTM_ERR_UNSUPPORTED, "grouped matmul: dtype %d is not supported (Float16, BFloat16 only)", dtype);
     if (N < 0 || K < 0) return set_error(BTM_ERR_INVALID, "grouped matmul: negative dimension (N=%d K=%d)", N, K);
     int rc = check_groups("grouped matmul", groups, rows, offsets);
+    if (!rc) rc = check_dims("grouped matmul", rows, N, K);
     if (rc) return rc;
     if (groups > 0 && rows > 0 && N > 0 && (!C || (K > 0 && (!A || !B)))) return set_error(BTM_ERR_INVALID, "grouped matmul: null pointer");
     const int64_t b_inner = b_transposed ? K : N, b_outer = b_transposed ? N : K;
@@ -782,6 +793,7 @@ int btm_gemm_grouped_wgrad(int device, void *stream, int dtype, int groups, int 
         return set_error(BTM_ERR_UNSUPPORTED, "grouped weight gradient: dtype %d is not supported (Float16, BFloat16 only)", dtype);
     if (M < 0 || N < 0) return set_error(BTM_ERR_INVALID, "grouped weight gradient: negative dimension (M=%d N=%d)", M, N);
     int rc = check_groups("grouped weight gradient", groups, rows, offsets);
+    if (!rc) rc = check_dims("grouped weight gradient", rows, M, N);
     if (rc) return rc;
     if (groups > 0 && M > 0 && N > 0 && (!C || (rows > 0 && (!A || !D)))) return set_error(BTM_ERR_INVALID, "grouped weight gradient: null pointer");
     if (lda < M || ldd < N || ldc < N)
@@ -810,6 +822,8 @@ static int check_mxfp4(const char *what, int groups, int rows, int K, const void
 {
     if (groups < 0 || rows < 0 || K < 0) return set_error(BTM_ERR_INVALID, "%s: negative dimension (groups=%d rows=%d K=%d)", what, groups, rows, K);
     if (K % 32) return set_error(BTM_ERR_INVALID, "%s: K=%d must be a multiple of 32", what, K);
+    if (int rc = check_dims(what, rows, K, 0)) return rc;
+    if (groups > kMaxGroups) return set_error(BTM_ERR_UNSUPPORTED, "%s: %d groups are more than the %d that are supported", what, groups, kMaxGroups);
     if (groups > 0 && rows > 0 && K > 0 && (!packed || !scales)) return set_error(BTM_ERR_INVALID, "%s: null pointer", what);
     if (((uintptr_t)packed | (uintptr_t)scales) & 15) return set_error(BTM_ERR_INVALID, "%s: packed values and scales must be 16-byte aligned", what);
     return BTM_OK;

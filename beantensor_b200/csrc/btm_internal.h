@@ -116,6 +116,8 @@ struct GroupedCall {
 int configure_gemm_grouped_kernels();
 int configure_gemm_grouped_pair_kernels();
 int configure_grouped_decode_kernels();
+int load_grouped_simt_kernels();
+int load_mxfp4_convert_kernels();
 bool grouped_decode_fits(int groups, int rows, int N, int sm_count);
 int launch_grouped_decode(const GroupedCall &c, cudaStream_t st, int sm_count, int *status);
 int launch_gemm_grouped_pair(const GroupedCall &c, cudaStream_t st, int sm_count, const CUtensorMap &tmA, const CUtensorMap &tmA_band,

@@ -411,6 +411,16 @@ static cudaError_t raise_grouped_smem()
     return e;
 }
 
+int load_grouped_simt_kernels()
+{
+    cudaFuncAttributes a;
+    cudaError_t e = cudaFuncGetAttributes(&a, gemm_grouped_simt_kernel<BTM_F16, true>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, gemm_grouped_simt_kernel<BTM_F16, false>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, gemm_grouped_simt_kernel<BTM_BF16, true>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, gemm_grouped_simt_kernel<BTM_BF16, false>);
+    return check_cuda(e, "cudaFuncGetAttributes(grouped general kernel)");
+}
+
 int configure_gemm_grouped_kernels()
 {
     cudaError_t e = raise_grouped_smem<BTM_F16>();

@@ -62,6 +62,8 @@ struct DecodeArgs {
     int *status;
     long long wait_limit;
     int skip_loads;
+    int debug_bounds;    // as GemmParams: hand-computed store addresses are compared with the extent of the output
+    long long extent;
 };
 
 template <int DT, int KIND>
@@ -293,7 +295,12 @@ __global__ void __launch_bounds__(dec::THREADS, 2) grouped_decode_kernel(const _
                 q[0] = *reinterpret_cast<const uint32_t *>(&h0);
                 q[1] = *reinterpret_cast<const uint32_t *>(&h1);
             }
-            uint16_t *dst = reinterpret_cast<uint16_t *>(a.out) + (long long)(m0 + c) * a.ldo + n;
+            const long long off = (long long)(m0 + c) * a.ldo + n;
+            uint16_t *dst = reinterpret_cast<uint16_t *>(a.out) + off;
+            if (a.debug_bounds && n < a.N && off + min(4, a.N - n) > a.extent) {
+                atomicCAS(a.status, 0, (int)BOUNDS_STORE);
+                continue;
+            }
             if (a.vec && n + 4 <= a.N) {
                 *reinterpret_cast<uint2 *>(dst) = make_uint2(q[0], q[1]);
             } else {
@@ -372,10 +379,13 @@ static int prepare(DecodeArgs *a, int rows, int groups, int N, int K, const int 
     a->vec = ((uintptr_t)out & 7) == 0 && ldo % 4 == 0;
     GemmParams p;
     memset(&p, 0, sizeof(p));
+    p.M = rows; p.N = N; p.batch = 1; p.ldc = ldo;
     fill_wait_params(&p);
     a->status = status;
     a->wait_limit = p.wait_limit;
     a->skip_loads = p.debug_skip_loads;
+    a->debug_bounds = p.debug_bounds;
+    a->extent = p.c_extent;
     const long long tiles = slot_bound(groups, rows) * a->n_blocks;
     // K over as many CTAs as two per SM leave room for.
     long long s = 2LL * sm_count / tiles;

@@ -364,4 +364,22 @@ int launch_mxfp4_dequant(cudaStream_t st, int dst_dtype, int groups, int rows, i
     return check_cuda(e, "mxfp4 dequantise launch");
 }
 
+template <typename T>
+static cudaError_t load_convert()
+{
+    cudaFuncAttributes a;
+    cudaError_t e = cudaFuncGetAttributes(&a, mxfp4_quantize_kernel<T, 1>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, mxfp4_quantize_kernel<T, 4>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, mxfp4_dequant_kernel<T>);
+    return e;
+}
+
+int load_mxfp4_convert_kernels()
+{
+    cudaError_t e = load_convert<float>();
+    if (e == cudaSuccess) e = load_convert<__half>();
+    if (e == cudaSuccess) e = load_convert<__nv_bfloat16>();
+    return check_cuda(e, "cudaFuncGetAttributes(mxfp4)");
+}
+
 } // namespace btm

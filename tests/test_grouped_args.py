@@ -135,3 +135,15 @@ def test_scale_bytes_of_both_sides_agree():
         for rows in (0, 1, 5, 127, 128, 129, 1000, 2 ** 31 - 1):
             for K in (0, 32, 128, 160, 4096):
                 assert ops.mxfp4_scale_bytes(rows, K, groups) == n(groups, rows, K)
+
+
+def test_sizes_beyond_the_kernels_are_refused():
+    L = _lib.lib()
+    big = 2 ** 31 - 1
+    refused(L.btm_gemm_grouped(0, None, _lib.F16, 2, big, 16, 32, OFF, P, 32, P, 512, 16, 0, P, 16), _lib.ERR_UNSUPPORTED, "dimensions")
+    refused(L.btm_gemm_grouped(0, None, _lib.F16, 2 ** 21, 8, 16, 32, OFF, P, 32, P, 512, 16, 0, P, 16), _lib.ERR_UNSUPPORTED, "groups")
+    refused(L.btm_gemm_grouped_wgrad(0, None, _lib.F16, 2, big, 32, 16, OFF, P, 32, P, 16, P, 512, 16), _lib.ERR_UNSUPPORTED, "dimensions")
+    refused(L.btm_mxfp4_quantize(0, None, _lib.F16, 1, big, 32, None, P, 32, P, P), _lib.ERR_UNSUPPORTED, "dimensions")
+    refused(L.btm_mxfp4_quantize(0, None, _lib.F16, 2 ** 21, 2 ** 21, 32, None, P, 32, P, P), _lib.ERR_UNSUPPORTED, "groups")
+    refused(L.btm_mxfp4_matmul(0, None, _lib.F16, big, 8, 32, P, P, P, P, P, 8), _lib.ERR_UNSUPPORTED, "dimensions")
+    refused(L.btm_mxfp4_matmul(0, None, _lib.F16, 8, big, 32, P, P, P, P, P, big), _lib.ERR_UNSUPPORTED, "dimensions")
