@@ -143,4 +143,146 @@ inline void matmul_int4_gpu(const btm_tensor_view &act, const btm_tensor_view &w
                               const_cast<void *>(btm_base(out))));
 }
 
+// A dimension as the C ABI takes it.
+inline int btm_dim(uint64_t n)
+{
+    if (n > 0x7FFFFFFFull) throw std::invalid_argument("dimension does not fit 32 bits");
+    return static_cast<int>(n);
+}
+
+// Row offsets of the groups: a rank-1 Int32 tensor of groups + 1 entries on the operands' GPU.
+inline const int32_t *btm_group_offsets(const btm_tensor_view &offsets, uint64_t groups, int32_t gpu_id, const char *name)
+{
+    btm_require_gpu_rowmajor(offsets, 1, name);
+    if (offsets.dtype != BTM_I32 || offsets.shape[0] != groups + 1 || offsets.gpu_id != gpu_id)
+        throw std::invalid_argument(std::string(name) + ": offsets must be an Int32 tensor of groups + 1 entries on the operands' GPU");
+    return static_cast<const int32_t *>(btm_base(offsets));
+}
+
+inline int64_t btm_pitch(const btm_tensor_view &t) // leading dimension of the last two dimensions; a single row has none of its own
+{
+    const uint64_t rows = t.shape[t.ndim - 2], cols = t.shape[t.ndim - 1];
+    return rows > 1 ? (int64_t)t.strides[t.ndim - 2] : (int64_t)(cols > 0 ? cols : 1);
+}
+
+// out[r,:] = a[r,:] . b[g] for the rows r of group g (offsets[g] <= r < offsets[g+1]); a [rows,K], b [groups,K,N], out [rows,N],
+// Float16/BFloat16. Each matrix of b may be transposed (b [groups,K,N] with unit stride along K): with the output gradient as
+// a this is the gradient of the activations. Rows outside the groups keep what out held.
+inline void grouped_matmul_gpu(const btm_tensor_view &a, const btm_tensor_view &b, const btm_tensor_view &offsets, btm_tensor_view &out,
+                               void *stream = nullptr)
+{
+    btm_require_gpu_rowmajor(a, 2, "grouped_matmul_gpu(a)");
+    btm_require_gpu_rowmajor(out, 2, "grouped_matmul_gpu(out)");
+    if (b.device != 1) throw std::invalid_argument("grouped_matmul_gpu(b): Tensor is not on the GPU");
+    if (b.ndim != 3) throw std::invalid_argument("grouped_matmul_gpu(b): wrong rank");
+    if (a.dtype != b.dtype || a.dtype != out.dtype) throw std::invalid_argument("grouped_matmul_gpu: dtypes differ");
+    if (a.gpu_id != b.gpu_id || a.gpu_id != out.gpu_id) throw std::invalid_argument("grouped_matmul_gpu: tensors live on different GPUs");
+    if (a.shape[1] != b.shape[1] || out.shape[0] != a.shape[0] || out.shape[1] != b.shape[2])
+        throw std::invalid_argument("grouped_matmul_gpu: shape mismatch");
+    const int32_t *offs = btm_group_offsets(offsets, b.shape[0], a.gpu_id, "grouped_matmul_gpu(offsets)");
+    const uint64_t K = b.shape[1], N = b.shape[2];
+    const bool trans = N > 1 && b.strides[2] != 1;
+    if (trans && K > 1 && b.strides[1] != 1) throw std::invalid_argument("grouped_matmul_gpu(b): each matrix must be row-major or transposed row-major");
+    const int64_t ldb = trans ? (int64_t)b.strides[2] : (K > 1 ? (int64_t)b.strides[1] : (int64_t)(N > 0 ? N : 1));
+    const int64_t sb = b.shape[0] > 1 ? (int64_t)b.strides[0] : ldb * (int64_t)(trans ? N : K);
+    btm_raise(btm_gemm_grouped(a.gpu_id, stream, a.dtype, btm_dim(b.shape[0]), btm_dim(a.shape[0]), btm_dim(N), btm_dim(K), offs, btm_base(a), btm_pitch(a), btm_base(b),
+                               sb, ldb, trans ? 1 : 0, const_cast<void *>(btm_base(out)), btm_pitch(out)));
+}
+
+// The weight gradient of the above: out[g] = a[rows of g]^T . dout[rows of g]; a [rows,K], dout [rows,N], out [groups,K,N].
+inline void grouped_matmul_wgrad_gpu(const btm_tensor_view &a, const btm_tensor_view &dout, const btm_tensor_view &offsets, btm_tensor_view &out,
+                                     void *stream = nullptr)
+{
+    btm_require_gpu_rowmajor(a, 2, "grouped_matmul_wgrad_gpu(a)");
+    btm_require_gpu_rowmajor(dout, 2, "grouped_matmul_wgrad_gpu(dout)");
+    btm_require_gpu_rowmajor(out, 3, "grouped_matmul_wgrad_gpu(out)");
+    if (a.dtype != dout.dtype || a.dtype != out.dtype) throw std::invalid_argument("grouped_matmul_wgrad_gpu: dtypes differ");
+    if (a.gpu_id != dout.gpu_id || a.gpu_id != out.gpu_id) throw std::invalid_argument("grouped_matmul_wgrad_gpu: tensors live on different GPUs");
+    if (a.shape[0] != dout.shape[0] || out.shape[1] != a.shape[1] || out.shape[2] != dout.shape[1])
+        throw std::invalid_argument("grouped_matmul_wgrad_gpu: shape mismatch");
+    const int32_t *offs = btm_group_offsets(offsets, out.shape[0], a.gpu_id, "grouped_matmul_wgrad_gpu(offsets)");
+    const int64_t ldc = btm_pitch(out);
+    const int64_t sc = out.shape[0] > 1 ? (int64_t)out.strides[0] : ldc * (int64_t)out.shape[1];
+    btm_raise(btm_gemm_grouped_wgrad(a.gpu_id, stream, a.dtype, btm_dim(out.shape[0]), btm_dim(a.shape[0]), btm_dim(out.shape[1]), btm_dim(out.shape[2]), offs, btm_base(a),
+                                     btm_pitch(a), btm_base(dout), btm_pitch(dout), const_cast<void *>(btm_base(out)), sc, ldc));
+}
+
+// A microscaled operand: packed [.., K/2] UInt8, dense, and its scale blocks, a rank-1 UInt8 tensor of at least `bytes`.
+inline void btm_require_mxfp4(const btm_tensor_view &packed, const btm_tensor_view &scales, int ndim, uint64_t bytes, const char *name)
+{
+    btm_require_gpu_rowmajor(packed, ndim, name);
+    btm_require_gpu_rowmajor(scales, 1, name);
+    if (packed.dtype != BTM_U8 || scales.dtype != BTM_U8) throw std::invalid_argument(std::string(name) + ": packed values and scales are UInt8");
+    if (scales.shape[0] < bytes) throw std::invalid_argument(std::string(name) + ": too few scale bytes");
+    uint64_t stride = 1;
+    for (int i = ndim - 1; i >= 0; --i) {
+        if (packed.shape[i] > 1 && packed.strides[i] != stride) throw std::invalid_argument(std::string(name) + ": packed values must be contiguous");
+        stride *= packed.shape[i];
+    }
+    if (packed.gpu_id != scales.gpu_id) throw std::invalid_argument(std::string(name) + ": tensors live on different GPUs");
+}
+
+// x [rows,K] (Float32/Float16/BFloat16) -> packed [rows,K/2] and scales; with offsets the scales are laid out for those groups.
+inline void quantize_mxfp4_gpu(const btm_tensor_view &x, btm_tensor_view &packed, btm_tensor_view &scales, const btm_tensor_view *offsets = nullptr,
+                               void *stream = nullptr)
+{
+    btm_require_gpu_rowmajor(x, 2, "quantize_mxfp4_gpu(x)");
+    const int groups = offsets ? btm_dim(offsets->shape[0]) - 1 : 1, rows = btm_dim(x.shape[0]), K = btm_dim(x.shape[1]);
+    btm_require_mxfp4(packed, scales, 2, btm_mxfp4_scale_bytes(groups, rows, K), "quantize_mxfp4_gpu(packed)");
+    if (packed.gpu_id != x.gpu_id || packed.shape[0] != x.shape[0] || packed.shape[1] * 2 != x.shape[1])
+        throw std::invalid_argument("quantize_mxfp4_gpu: shape mismatch");
+    const int32_t *offs = offsets ? btm_group_offsets(*offsets, (uint64_t)groups, x.gpu_id, "quantize_mxfp4_gpu(offsets)") : nullptr;
+    btm_raise(btm_mxfp4_quantize(x.gpu_id, stream, x.dtype, groups, rows, K, offs, btm_base(x), btm_pitch(x), const_cast<void *>(btm_base(packed)),
+                                 const_cast<void *>(btm_base(scales))));
+}
+
+// The inverse: out [rows,K] = the values that packed and scales stand for, rounded once to out's dtype.
+inline void dequant_mxfp4_gpu(const btm_tensor_view &packed, const btm_tensor_view &scales, btm_tensor_view &out, const btm_tensor_view *offsets = nullptr,
+                              void *stream = nullptr)
+{
+    btm_require_gpu_rowmajor(out, 2, "dequant_mxfp4_gpu(out)");
+    const int groups = offsets ? btm_dim(offsets->shape[0]) - 1 : 1, rows = btm_dim(out.shape[0]), K = btm_dim(out.shape[1]);
+    btm_require_mxfp4(packed, scales, 2, btm_mxfp4_scale_bytes(groups, rows, K), "dequant_mxfp4_gpu(packed)");
+    if (packed.gpu_id != out.gpu_id || packed.shape[0] != out.shape[0] || packed.shape[1] * 2 != out.shape[1])
+        throw std::invalid_argument("dequant_mxfp4_gpu: shape mismatch");
+    const int32_t *offs = offsets ? btm_group_offsets(*offsets, (uint64_t)groups, out.gpu_id, "dequant_mxfp4_gpu(offsets)") : nullptr;
+    btm_raise(btm_mxfp4_dequant(out.gpu_id, stream, out.dtype, groups, rows, K, offs, btm_base(packed), btm_base(scales), const_cast<void *>(btm_base(out)),
+                                btm_pitch(out)));
+}
+
+// out[M,N] (Float16/BFloat16) = act[M,K] . w[N,K]^T of microscaled operands.
+inline void matmul_mxfp4_gpu(const btm_tensor_view &act, const btm_tensor_view &act_scales, const btm_tensor_view &w, const btm_tensor_view &w_scales,
+                             btm_tensor_view &out, void *stream = nullptr)
+{
+    btm_require_gpu_rowmajor(act, 2, "matmul_mxfp4_gpu(act)");
+    btm_require_gpu_rowmajor(w, 2, "matmul_mxfp4_gpu(w)");
+    btm_require_gpu_rowmajor(out, 2, "matmul_mxfp4_gpu(out)");
+    const int M = btm_dim(act.shape[0]), N = btm_dim(w.shape[0]), K = btm_dim(act.shape[1] * 2);
+    btm_require_mxfp4(act, act_scales, 2, btm_mxfp4_scale_bytes(1, M, K), "matmul_mxfp4_gpu(act)");
+    btm_require_mxfp4(w, w_scales, 2, btm_mxfp4_scale_bytes(1, N, K), "matmul_mxfp4_gpu(w)");
+    if (w.shape[1] != act.shape[1] || out.shape[0] != act.shape[0] || out.shape[1] != w.shape[0])
+        throw std::invalid_argument("matmul_mxfp4_gpu: shape mismatch");
+    if (act.gpu_id != w.gpu_id || act.gpu_id != out.gpu_id) throw std::invalid_argument("matmul_mxfp4_gpu: tensors live on different GPUs");
+    btm_raise(btm_mxfp4_matmul(act.gpu_id, stream, out.dtype, M, N, K, btm_base(act), btm_base(act_scales), btm_base(w), btm_base(w_scales),
+                               const_cast<void *>(btm_base(out)), btm_pitch(out)));
+}
+
+// out[r,:] = act[r,:] . w[g]^T for the rows r of group g; act [rows,K/2] quantised with these offsets, w [groups,N,K/2].
+inline void grouped_matmul_mxfp4_gpu(const btm_tensor_view &act, const btm_tensor_view &act_scales, const btm_tensor_view &w,
+                                     const btm_tensor_view &w_scales, const btm_tensor_view &offsets, btm_tensor_view &out, void *stream = nullptr)
+{
+    btm_require_gpu_rowmajor(act, 2, "grouped_matmul_mxfp4_gpu(act)");
+    btm_require_gpu_rowmajor(w, 3, "grouped_matmul_mxfp4_gpu(w)");
+    btm_require_gpu_rowmajor(out, 2, "grouped_matmul_mxfp4_gpu(out)");
+    const int groups = btm_dim(w.shape[0]), rows = btm_dim(act.shape[0]), N = btm_dim(w.shape[1]), K = btm_dim(act.shape[1] * 2);
+    btm_require_mxfp4(act, act_scales, 2, btm_mxfp4_scale_bytes(groups, rows, K), "grouped_matmul_mxfp4_gpu(act)");
+    btm_require_mxfp4(w, w_scales, 3, (uint64_t)groups * btm_mxfp4_scale_bytes(1, N, K), "grouped_matmul_mxfp4_gpu(w)");
+    if (w.shape[2] != act.shape[1] || out.shape[0] != act.shape[0] || out.shape[1] != w.shape[1])
+        throw std::invalid_argument("grouped_matmul_mxfp4_gpu: shape mismatch");
+    if (act.gpu_id != w.gpu_id || act.gpu_id != out.gpu_id) throw std::invalid_argument("grouped_matmul_mxfp4_gpu: tensors live on different GPUs");
+    const int32_t *offs = btm_group_offsets(offsets, (uint64_t)groups, act.gpu_id, "grouped_matmul_mxfp4_gpu(offsets)");
+    btm_raise(btm_mxfp4_matmul_grouped(act.gpu_id, stream, out.dtype, groups, rows, N, K, offs, btm_base(act), btm_base(act_scales), btm_base(w),
+                                       btm_base(w_scales), const_cast<void *>(btm_base(out)), btm_pitch(out)));
+}
+
 } // namespace BeanTensor::Tensors::detail

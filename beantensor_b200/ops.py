@@ -210,6 +210,11 @@ def _bad_offsets(what: str) -> None:
     raise ValueError(f"{what}: offsets must be a contiguous Int32 tensor of groups + 1 entries")
 
 
+def _too_large(what: str) -> None:
+    from .errors import NotImplementedOp
+    raise NotImplementedOp(f"{what}: dimensions must fit 32 bits")
+
+
 def _row_pitch(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
     """Leading dimension of a row-major matrix, the last two dimensions of t; a single row has none of its own."""
     st = t.stride()
@@ -243,6 +248,8 @@ def grouped_matmul_gpu(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, 
         raise ValueError(f"grouped_matmul_gpu: shape mismatch {tuple(sa)} x {tuple(sb)} -> {tuple(out.shape)}")
     if offsets.dtype != _I32 or offsets.shape != (G + 1,) or not offsets.is_contiguous():
         _bad_offsets("grouped_matmul_gpu")
+    if (rows | N | K | G) >> 31:
+        _too_large("grouped_matmul_gpu")
     lda, ldc = _row_pitch(a, rows, K, "a"), _row_pitch(out, rows, N, "out")
     bg, bk, bn = b.stride()
     trans = bn != 1 and N > 1
@@ -281,6 +288,8 @@ def grouped_matmul_wgrad_gpu(a: torch.Tensor, dout: torch.Tensor, offsets: torch
         raise ValueError(f"grouped_matmul_wgrad_gpu: shape mismatch {tuple(sa)} x {tuple(sd)} -> {tuple(out.shape)}")
     if offsets.dtype != _I32 or offsets.shape != (G + 1,) or not offsets.is_contiguous():
         _bad_offsets("grouped_matmul_wgrad_gpu")
+    if (rows | N | K | G) >> 31:
+        _too_large("grouped_matmul_wgrad_gpu")
     lda, ldd, ldc = _row_pitch(a, rows, K, "a"), _row_pitch(dout, rows, N, "dout"), _row_pitch(out, K, N, "out")
     rc = _LIB().btm_gemm_grouped_wgrad(dev, _raw_stream(dev), dt, G, rows, K, N, offsets.data_ptr(), a.data_ptr(), lda, dout.data_ptr(), ldd,
                                        out.data_ptr(), out.stride(0) if G > 1 else K * ldc, ldc)
@@ -338,6 +347,8 @@ def _mxfp4_convert(fn, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tens
         raise ValueError(f"{what} takes 2-D or 3-D tensors")
     if not fits or K % 32 or packed.dtype != _U8 or scales.dtype != _U8 or not packed.is_contiguous() or not scales.is_contiguous():
         _bad_mxfp4(packed, scales, K, what, fits)
+    if (rows | K | groups) >> 31:
+        _too_large(what)
     if quantize:
         rc = fn(dev, _raw_stream(dev), dt, groups, rows, K, table, x.data_ptr(), ld, packed.data_ptr(), scales.data_ptr())
     else:
@@ -385,6 +396,8 @@ def matmul_mxfp4_gpu(act: torch.Tensor, act_scales: torch.Tensor, w: torch.Tenso
     K = 2 * half
     if half != half2 or out.shape != (M, N) or act_scales.numel() < mxfp4_scale_bytes(M, K) or w_scales.numel() < mxfp4_scale_bytes(N, K):
         raise ValueError("matmul_mxfp4_gpu: shape mismatch")
+    if (M | N | K) >> 31:
+        _too_large("matmul_mxfp4_gpu")
     dt = _mxfp4_product_dtype("matmul_mxfp4_gpu", act, act_scales, w, w_scales, out, K)
     rc = _LIB().btm_mxfp4_matmul(dev, _raw_stream(dev), dt, M, N, K, act.data_ptr(), act_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(),
                                  out.data_ptr(), _row_pitch(out, M, N, "out"))
@@ -409,6 +422,8 @@ def grouped_matmul_mxfp4_gpu(act: torch.Tensor, act_scales: torch.Tensor, w: tor
         raise ValueError("grouped_matmul_mxfp4_gpu: shape mismatch")
     if offsets.dtype != _I32 or offsets.shape != (G + 1,) or not offsets.is_contiguous():
         _bad_offsets("grouped_matmul_mxfp4_gpu")
+    if (rows | N | K | G) >> 31:
+        _too_large("grouped_matmul_mxfp4_gpu")
     dt = _mxfp4_product_dtype("grouped_matmul_mxfp4_gpu", act, act_scales, w, w_scales, out, K)
     rc = _LIB().btm_mxfp4_matmul_grouped(dev, _raw_stream(dev), dt, G, rows, N, K, offsets.data_ptr(), act.data_ptr(), act_scales.data_ptr(),
                                          w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), _row_pitch(out, rows, N, "out"))
