@@ -209,7 +209,8 @@ int btm_bmm(int device, void *stream, int dtype, int batch, int M, int N, int K,
  * Ordering: the products use programmatic dependent launch. If the preceding kernel on the
  * stream is another int4 product of this library, this one may read w_packed and scales_f16 while
  * that kernel is still running (act_f16 is read and out_f16 written only after it has completed);
- * w_packed and scales_f16 must therefore not be the output of an immediately preceding int4 product. */
+ * w_packed and scales_f16 must therefore not be the output of an immediately preceding int4 product, nor of a
+ * grouped or microscaled call (below), which let their successor in early too. */
 int btm_int4_matmul(int device, void *stream, int M, int N, int K, int group, const void *act_f16,
                     const void *w_packed, const void *scales_f16, void *out_f16);
 
