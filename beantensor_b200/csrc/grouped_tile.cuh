@@ -196,7 +196,9 @@ __device__ __forceinline__ void grouped_band(const GemmParams &p, const CUtensor
             for (int j = 0; j < 4; ++j)
                 st_shared_v4(buf + (uint32_t)lane * 128u + (((uint32_t)(h * 4 + j) ^ swz) << 4), q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
         }
-        if (whole) {
+        // A TMA store clips rows where the matrix ends, but columns only to whole 16 bytes: up to seven values behind N, which may
+        // be another matrix's columns, would be overwritten with zeros. Chunks that end inside 16 bytes go the other way.
+        if (whole && (col + 64 <= p.N || (p.N & 7) == 0)) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {

@@ -215,3 +215,37 @@ def test_side_stream_orders_by_itself(btm):
                 exact, mass = ragged.product(ragged.quantize(a[lo:hi])[0], ragged.quantize(b[g].t().contiguous())[0].t())
                 ragged.check(o4[lo:hi], exact, mass, K)
     btm.check_device_status(0)
+
+
+@pytest.mark.parametrize("kernel", ["1cta", "2cta", "decode"])
+@pytest.mark.parametrize("N", [1, 5, 37, 61, 66, 130, 325])
+def test_columns_behind_an_odd_width_are_kept(btm, monkeypatch, kernel, N):
+    # The output's pitch is a multiple of 16 bytes, its width is not: what lies between belongs to somebody else.
+    monkeypatch.setenv("BTM_FORCE_KERNEL", kernel)
+    rows, K, pitch = 200, 128, (N + 7) // 8 * 8
+    bounds = [0, 64, 64, 190]
+    t = table(bounds)
+    a, d = normal((rows, K), BF16, 1), normal((rows, pitch), BF16, 2)[:, :N]
+    b = normal((3, K, pitch), BF16, 3)[:, :, :N]
+    wide, grad = normal((rows, pitch), BF16, 4), normal((3, K, pitch), BF16, 5)
+    kept, kept_grad = wide.clone(), grad.clone()
+    btm.grouped_matmul_gpu(a, b, t, wide[:, :N])
+    btm.grouped_matmul_wgrad_gpu(a, d, t, grad[:, :, :N])
+    btm.check_device_status(0)
+    for g, (lo, hi) in enumerate(ragged.spans(bounds, rows)):
+        if hi > lo:
+            ragged.check(wide[lo:hi, :N], *ragged.product(a[lo:hi], b[g]), K)
+        ragged.check(grad[g, :, :N], *ragged.product(a[lo:hi].t(), d[lo:hi]), hi - lo)
+    assert torch.equal(wide[:, N:], kept[:, N:]) and torch.equal(grad[:, :, N:], kept_grad[:, :, N:]) and torch.equal(wide[190:], kept[190:])
+    xq, xs = quantized(btm, a, t, 3)
+    w = b.transpose(1, 2).contiguous()
+    wq = torch.empty((3, N, K // 2), dtype=torch.uint8, device="cuda")
+    ws = torch.empty((3, btm.mxfp4_scale_bytes(N, K)), dtype=torch.uint8, device="cuda")
+    btm.quantize_mxfp4_gpu(w, wq, ws)
+    wide = kept.clone()
+    btm.grouped_matmul_mxfp4_gpu(xq, xs, wq, ws, t, wide[:, :N])
+    btm.check_device_status(0)
+    for g, (lo, hi) in enumerate(ragged.spans(bounds, rows)):
+        if hi > lo:
+            ragged.check(wide[lo:hi, :N], *ragged.product(ragged.quantize(a[lo:hi])[0], ragged.quantize(w[g])[0].t()), K)
+    assert torch.equal(wide[:, N:], kept[:, N:]) and torch.equal(wide[190:], kept[190:])
