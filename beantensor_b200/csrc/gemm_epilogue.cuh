@@ -4,10 +4,13 @@
 // band of the tile. It reads 32 accumulator columns at a time with tcgen05.ld, rounds to the output
 // type and writes them into a warp-private shared-memory tile of 32 rows x 128 bytes laid out with
 // the 128-byte swizzle (conflict-free 16-byte stores); one lane then hands the tile to a TMA store
-// (cp.async.bulk.tensor ... global.shared::cta). The TMA unit clips
-// rows and columns beyond the matrix, so the band needs no predicates, and C is written in whole
-// 128-byte lines. Two tiles per warp alternate so that a store drains while the next is filled. With
-// several destination copies of C the peers are written by epilogue_band_multi (below).
+// (cp.async.bulk.tensor ... global.shared::cta). The TMA unit clips rows beyond the matrix, so the band
+// needs no predicates, and C is written in whole 128-byte lines. Columns it clips only to whole 16
+// bytes: up to seven values behind an N that ends inside them would be overwritten with zeros, and in a
+// wider pitch they are somebody else's. A staging tile that ends so is stored element by element
+// (store_cut_tile); there is one per row of tiles at most. Two tiles per warp alternate so that a store
+// drains while the next is filled. With several destination copies of C the peers are written by
+// epilogue_band_multi (below).
 // General path (unaligned C): per-thread row stores, as the kernels did originally.
 #pragma once
 #include <cuda_bf16.h>
@@ -124,6 +127,37 @@ __device__ __forceinline__ void store_row_direct(const GemmParams &p, const uint
     }
 }
 
+// Does the staging tile whose first column is `col` end inside 16 bytes of C? (C itself, its pitch and col0 are multiples of 16.)
+template <int DT>
+__device__ __forceinline__ bool tile_is_cut(const GemmParams &p, int col)
+{
+    constexpr int kUnit = DT == BTM_F32 ? 4 : 8, kCols = DT == BTM_F32 ? 32 : 64;
+    return col < p.N && col + kCols > p.N && (p.N & (kUnit - 1)) != 0;
+}
+
+// Such a tile to the local copy of C, a row at a time: lane l holds 4 bytes of it. The caller has synchronised the warp behind
+// the writes of the tile.
+template <int DT>
+__device__ __forceinline__ void store_cut_tile(const GemmParams &p, uint32_t buf, int row0, int col, int batch, int lane)
+{
+    const int cols = p.N - col, rows = min(32, p.M - row0);
+    const long long base = (long long)batch * p.strideC + (long long)row0 * p.ldc + p.col0 + col;
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+        const long long off = base + (long long)r * p.ldc;
+        if (!store_in_bounds(p, off, cols)) return;
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(buf + (uint32_t)r * 128u + ((((uint32_t)lane >> 2) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(lane & 3) * 4u));
+        if constexpr (DT == BTM_F32) {
+            if (lane < cols) reinterpret_cast<uint32_t *>(p.C[0])[off + lane] = w;
+        } else {
+            uint16_t *dst = reinterpret_cast<uint16_t *>(p.C[0]) + off + 2 * lane;
+            if (2 * lane < cols) dst[0] = (uint16_t)w;
+            if (2 * lane + 1 < cols) dst[1] = (uint16_t)(w >> 16);
+        }
+    }
+}
+
 // Band drain when C has several destination copies (the fused all-gather of the N-sharded product).
 // 128 output columns at a time: both staging tiles are filled, the local copy goes out as two TMA
 // stores, and the peers are written with plain 16-byte stores from registers, laid out so that one
@@ -167,10 +201,14 @@ __device__ __forceinline__ void epilogue_band_multi(const GemmParams &p, const S
         const int col = col_first + c * 128;
         // With a multicast mapping the local copy is written by the same multimem stores as the peers' (this device
         // is a member of the object), so the staging tiles only serve the transposition below.
-        if (lane == 0 && p.mc == nullptr) {
-            if (row0 < p.M && col < p.N) tma_store_3d(&cmaps.m[0], epi_smem, (int)p.col0 + col, row0, batch);
-            if (row0 < p.M && col + 64 < p.N) tma_store_3d(&cmaps.m[0], epi_smem + EPI_TILE_BYTES, (int)p.col0 + col + 64, row0, batch);
-            bulk_commit();
+        if (p.mc == nullptr) {
+            const bool cut0 = tile_is_cut<DT>(p, col), cut1 = tile_is_cut<DT>(p, col + 64);
+            if (lane == 0) {
+                if (row0 < p.M && col < p.N && !cut0) tma_store_3d(&cmaps.m[0], epi_smem, (int)p.col0 + col, row0, batch);
+                if (row0 < p.M && col + 64 < p.N && !cut1) tma_store_3d(&cmaps.m[0], epi_smem + EPI_TILE_BYTES, (int)p.col0 + col + 64, row0, batch);
+                bulk_commit();
+            }
+            if (cut0 || cut1) store_cut_tile<DT>(p, epi_smem + (cut1 ? EPI_TILE_BYTES : 0), row0, cut1 ? col + 64 : col, batch, lane);
         }
         // Peers: lane l owns the 16-byte chunk (l & 15) of the 256-byte row pieces of rows 2 i + (l >> 4).
         const int chunk = lane & 15, tsel = chunk >> 3, cj = chunk & 7;
@@ -283,10 +321,12 @@ __device__ __forceinline__ void epilogue_band(const GemmParams &p, const StoreMa
         fence_proxy_async_smem(); // generic-proxy writes above -> visible to the TMA unit
         __syncwarp();
         const int col = col_first + c * kColsPerTile;
+        const bool cut = tile_is_cut<DT>(p, col);
         if (lane == 0) {
-            if (row0 < p.M && col < p.N) tma_store_3d(&cmaps.m[0], buf, (int)p.col0 + col, row0, batch);
+            if (row0 < p.M && col < p.N && !cut) tma_store_3d(&cmaps.m[0], buf, (int)p.col0 + col, row0, batch);
             bulk_commit(); // an empty group when nothing was stored keeps the buffer accounting uniform
         }
+        if (cut) store_cut_tile<DT>(p, buf, row0, col, batch, lane);
     }
 }
 
