@@ -110,8 +110,8 @@ DeviceState *device_state(int device)
         return nullptr;
     }
     if (ensure_encode()) return nullptr;
-    if (check_cuda(cudaMalloc(&ds->status, sizeof(int)), "cudaMalloc(status)")) return nullptr;
-    if (check_cuda(cudaMemset(ds->status, 0, sizeof(int)), "cudaMemset(status)")) return nullptr;
+    if (check_cuda(cudaMalloc(&ds->status, STATUS_WORDS * sizeof(int)), "cudaMalloc(status)")) return nullptr;
+    if (check_cuda(cudaMemset(ds->status, 0, STATUS_WORDS * sizeof(int)), "cudaMemset(status)")) return nullptr;
     // Scratch of the fp32 product comes from a pool of this library's own, in stream order. The release
     // threshold keeps freed blocks in the pool, so that after the first call of a shape an allocation is a
     // bookkeeping step on the host and not a trip to the driver.
@@ -394,21 +394,21 @@ int btm_check_device_status(int device, void *stream)
     DeviceState *ds = device_state(device);
     if (!ds) return last_code();
     cudaStream_t st = (cudaStream_t)stream;
-    int host = 0;
-    int rc = check_cuda(cudaMemcpyAsync(&host, ds->status, sizeof(int), cudaMemcpyDeviceToHost, st), "status readback");
+    int host[STATUS_WORDS] = {};
+    int rc = check_cuda(cudaMemcpyAsync(host, ds->status, sizeof(host), cudaMemcpyDeviceToHost, st), "status readback");
     if (rc) return rc;
     rc = check_cuda(cudaStreamSynchronize(st), "cudaStreamSynchronize");
     if (rc) return rc;
-    if (host != 0) {
-        cudaMemsetAsync(ds->status, 0, sizeof(int), st);
-        cudaStreamSynchronize(st);
-        if (host == 201)
-            return set_error(BTM_ERR_CUDA, "CUDA Error: a debug bounds check stopped a store outside the output (device status %d)", host);
-        if (host == 202)
-            return set_error(BTM_ERR_INVALID, "grouped operator: row offsets decrease or leave the rows (they were clamped; device status %d)", host);
-        return set_error(BTM_ERR_TIMEOUT, "CUDA Error: a kernel wait ran out (device status %d)", host);
-    }
-    return BTM_OK;
+    // One report per call, what made a kernel give up first; only the word that is reported is cleared.
+    const int word = host[0] != 0 ? 0 : STATUS_OFFSETS_WORD, code = host[word];
+    if (code == 0) return BTM_OK;
+    cudaMemsetAsync(ds->status + word, 0, sizeof(int), st);
+    cudaStreamSynchronize(st);
+    if (word == STATUS_OFFSETS_WORD)
+        return set_error(BTM_ERR_INVALID, "grouped operator: row offsets decrease or leave the rows (they were clamped; device status %d)", code);
+    if (code == 201)
+        return set_error(BTM_ERR_CUDA, "CUDA Error: a debug bounds check stopped a store outside the output (device status %d)", code);
+    return set_error(BTM_ERR_TIMEOUT, "CUDA Error: a kernel wait ran out (device status %d)", code);
 }
 
 static int gemm_entry(int device, void *stream, int dtype, int M, int N, int K, const void *A, int64_t lda, const void *B, int64_t ldb,

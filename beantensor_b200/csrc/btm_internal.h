@@ -47,11 +47,15 @@ struct StoreMaps {
     CUtensorMap m[kMaxDst];
 };
 
+// The device status is two words: the code of what made a kernel give up (the first one stays), and apart from it that a table
+// of row offsets had to be repaired.
+constexpr int STATUS_OFFSETS_WORD = 1, STATUS_WORDS = 2;
+
 // Per-device state, created once by btm_init.
 struct DeviceState {
     std::atomic<bool> ready;
     int sm_count;
-    int *status;        // device memory, one int
+    int *status;        // device memory, STATUS_WORDS ints
     cudaMemPool_t pool; // scratch of the fp32 split: allocated and freed in stream order, one block per call
 };
 

@@ -3,8 +3,8 @@
 // The table is written by the GPU (a router's counts), so the host never sees it: it sizes a launch from bounds, and
 // every warp that needs to know which rows a tile covers walks the table itself, 32 groups at a time, one per lane.
 // Nothing in the table can lead outside the operands: an entry is clamped to [0, rows], and one that is smaller than an
-// earlier one counts as that earlier one (its group is empty). A table that needed such repair is reported through the
-// device status word (ROWS_OFFSETS).
+// earlier one counts as that earlier one (its group is empty). A table that needed such repair is reported through a
+// device status word of its own (report_repaired).
 #pragma once
 #include "btm_internal.h"
 #include "btm_ptx.cuh"
@@ -13,6 +13,10 @@ namespace btm {
 
 constexpr int GROUP_SLOT_ROWS = 128; // a group's rows are cut into slots, the last one short: of so many rows, or twice
                                      // as many for a pair of CTAs
+
+// To the word behind the one that waits and bounds checks report to: a repaired table is no failure of the kernel, and must
+// neither hide one nor be hidden by it.
+__device__ __forceinline__ void report_repaired(int *status) { status[STATUS_OFFSETS_WORD] = ROWS_OFFSETS; }
 
 // All members are used by a whole warp at once. Without a table there is one group that owns every row.
 template <int kSlot = GROUP_SLOT_ROWS>
@@ -116,7 +120,7 @@ struct GroupWalk {
     // Reports a repaired table once (call after count_slots, from one warp of the grid).
     __device__ __forceinline__ void report(int *status) const
     {
-        if (bad) atomicCAS(status, 0, (int)ROWS_OFFSETS);
+        if (bad) report_repaired(status);
     }
 };
 

@@ -88,7 +88,7 @@ __device__ __forceinline__ SlotRows slot_rows(int slot, const int *offsets, int 
         floor_slot = total;
     }
     __syncthreads();
-    if (blockIdx.x == 0 && bad) atomicCAS(status, 0, (int)ROWS_OFFSETS);
+    if (blockIdx.x == 0 && bad) report_repaired(status);
     return found;
 }
 

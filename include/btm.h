@@ -111,9 +111,10 @@ int btm_debug_set(const char *key, long long value);
  * device checks (Tensor/TensorOps.cu:236-247). */
 int btm_init(int device);
 
-/* Reads and clears the device-side status word that kernels set when one of their
- * bounded waits ran out, or when a table of row offsets had to be repaired (btm_gemm_grouped). Synchronises
- * `stream`. Returns BTM_OK, BTM_ERR_TIMEOUT or BTM_ERR_INVALID. */
+/* Reads and clears the device-side status that kernels set when one of their bounded waits ran out
+ * (BTM_ERR_TIMEOUT) or a debug bounds check stopped a store (BTM_ERR_CUDA), or when a table of row offsets had to be
+ * repaired (BTM_ERR_INVALID, btm_gemm_grouped). Where both kinds happened the failure is returned first and the repaired
+ * table by the call after it. Synchronises `stream`. Returns BTM_OK when nothing is left to report. */
 int btm_check_device_status(int device, void *stream);
 
 /* Dense matmul C[M,N] = A[M,K] . B[K,N], the op that Ops/Algebra/MatMul/MatMul.h:1-8
