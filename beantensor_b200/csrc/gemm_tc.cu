@@ -295,12 +295,22 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     }
 }
 
-// Low part of the split. For an infinite x the high part is already x and x - hi would be Inf - Inf = NaN, which
-// would turn a whole output row or column into NaN where an fp32 product gives +-Inf; the low part is 0 there.
-__device__ __forceinline__ float split_lo(float x, float hi) { return fabsf(x) == INFINITY ? 0.0f : x - hi; }
-
 // 3xTF32 operand preparation: hi = x with the low 13 mantissa bits cleared (what the tensor
 // core reads of an fp32 word), lo = x - hi (exact in fp32). Written as two dense planes.
+//
+// An infinite x has no such low half. With hi = x the term hi . lo' would be Inf times the other factor's low half, NaN
+// wherever that is 0 (every value that TF32 holds whole). So its halves are a finite +-1 and x itself: hi . hi' and hi . lo'
+// are then finite for a finite factor y and lo . hi' is Inf times hi(y), which has the sign of y and is 0 only with y (or in
+// the last 13 bits of the subnormal range). Two infinities give +-Inf in both mixed terms, with the same sign, and 0 and NaN
+// give NaN, as in a plain product.
+__device__ __forceinline__ void split_tf32(float x, float &hi, float &lo)
+{
+    const bool inf = fabsf(x) == INFINITY;
+    const float h = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
+    hi = inf ? copysignf(1.0f, x) : h;
+    lo = inf ? x : x - h;
+}
+
 __global__ void split_tf32_kernel(const float *__restrict__ src, long long ld, int rows, int cols,
                                   float *__restrict__ hi, float *__restrict__ lo, long long ld_dst)
 {
@@ -310,9 +320,7 @@ __global__ void split_tf32_kernel(const float *__restrict__ src, long long ld, i
         const long long r = i / ld_dst;
         const int c = (int)(i - r * ld_dst);
         float x = (c < cols) ? src[r * ld + c] : 0.0f;
-        const float h = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
-        hi[i] = h;
-        lo[i] = split_lo(x, h);
+        split_tf32(x, hi[i], lo[i]);
     }
 }
 
@@ -333,9 +341,7 @@ __global__ void split_tf32_transpose_kernel(const float *__restrict__ src, long 
         const int c = c0 + i, r = r0 + threadIdx.x; // output row = source column
         if (c < cols && r < ld_dst) {
             const float x = tile[threadIdx.x][i];
-            const float h = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
-            hi[(long long)c * ld_dst + r] = h;
-            lo[(long long)c * ld_dst + r] = split_lo(x, h);
+            split_tf32(x, hi[(long long)c * ld_dst + r], lo[(long long)c * ld_dst + r]);
         }
     }
 }
@@ -355,9 +361,7 @@ __global__ void split_tf32_pair_kernel(const float *__restrict__ A, long long ld
             const int r = r0 + i, c = c0 + threadIdx.x;
             if (r < M && c < Kp) {
                 const float x = c < K ? A[(long long)r * lda + c] : 0.0f;
-                const float h = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
-                a_hi[(long long)r * Kp + c] = h;
-                a_lo[(long long)r * Kp + c] = split_lo(x, h);
+                split_tf32(x, a_hi[(long long)r * Kp + c], a_lo[(long long)r * Kp + c]);
             }
         }
         return;
@@ -373,9 +377,7 @@ __global__ void split_tf32_pair_kernel(const float *__restrict__ A, long long ld
         const int c = c0 + i, r = r0 + threadIdx.x;
         if (c < N && r < Kp) {
             const float x = tile[threadIdx.x][i];
-            const float h = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
-            b_hi[(long long)c * Kp + r] = h;
-            b_lo[(long long)c * Kp + r] = split_lo(x, h);
+            split_tf32(x, b_hi[(long long)c * Kp + r], b_lo[(long long)c * Kp + r]);
         }
     }
 }
