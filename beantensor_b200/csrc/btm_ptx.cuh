@@ -205,6 +205,17 @@ __device__ __forceinline__ bool mbar_wait_uniform(uint32_t bar, uint32_t parity,
 __device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
+// ---------------------------------------------------------------- programmatic dependent launch
+// 16 bytes that the kernel before may have written, read behind griddepcontrol.wait. This kernel may be running while they
+// are written, so they must not be read as data that never changes (const __restrict__, __ldg): such a load may be served
+// without regard to the wait, or be moved in front of it.
+__device__ __forceinline__ uint4 ld_dependent(const uint4 *p)
+{
+    uint4 v;
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *m)
 {

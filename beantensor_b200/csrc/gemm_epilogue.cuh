@@ -81,9 +81,9 @@ __device__ __forceinline__ void bias_act(const GemmParams &p, uint32_t (&v)[32],
     if (p.bias == nullptr && p.act == 0) return;
     float b = 0.0f;
     if (p.bias != nullptr && col + lane < p.N) {
-        if constexpr (DT == BTM_F32) b = __ldg(reinterpret_cast<const float *>(p.bias) + col + lane);
-        else if constexpr (DT == BTM_F16) b = __half2float(__ldg(reinterpret_cast<const __half *>(p.bias) + col + lane));
-        else b = __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16 *>(p.bias) + col + lane));
+        if constexpr (DT == BTM_F32) b = reinterpret_cast<const float *>(p.bias)[col + lane];
+        else if constexpr (DT == BTM_F16) b = __half2float(reinterpret_cast<const __half *>(p.bias)[col + lane]);
+        else b = __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p.bias)[col + lane]);
     }
 #pragma unroll
     for (int j = 0; j < 32; ++j) {

@@ -92,7 +92,7 @@ constexpr int GEMV_MAX_PIECES = 64;   // K <= 16384 on the fast GEMV path
 
 template <bool kStageAct>
 __global__ void __launch_bounds__(GEMV_WARPS * 32, 5)
-int4_gemv_kernel(const __grid_constant__ CUtensorMap tmW, int M, int N, int K, int group, const __half *__restrict__ act,
+int4_gemv_kernel(const __grid_constant__ CUtensorMap tmW, int M, int N, int K, int group, const __half *act,
                  const __half *__restrict__ scales, __half *__restrict__ out, int *status)
 {
     // The CTA's whole weight slab (16 rows x K/2 bytes) is requested from HBM at once: one tiled TMA load
@@ -169,7 +169,7 @@ int4_gemv_kernel(const __grid_constant__ CUtensorMap tmW, int M, int N, int K, i
         for (int j = 0; j < ACT_PRE; ++j) {
             const int i = threadIdx.x + j * blockDim.x;
             // rows m0.. of act are contiguous: uint4 index i of the span
-            if (i < act_total) act_pre[j] = __ldg(reinterpret_cast<const uint4 *>(act + (size_t)m0 * K) + i);
+            if (i < act_total) act_pre[j] = ld_dependent(reinterpret_cast<const uint4 *>(act + (size_t)m0 * K) + i);
         }
     }
     // 8 consecutive activations -> {k0,k4}, {k1,k5}, {k2,k6}, {k3,k7}: the slot order of the unpacked weights
@@ -196,7 +196,7 @@ int4_gemv_kernel(const __grid_constant__ CUtensorMap tmW, int M, int N, int K, i
             if (i < act_total) act_s[i + (i >= K / 8 ? 1 : 0)] = permute8(act_pre[j]);
         }
         for (int i = threadIdx.x + ACT_PRE * blockDim.x; i < act_total; i += blockDim.x)
-            act_s[i + (i >= K / 8 ? 1 : 0)] = permute8(__ldg(reinterpret_cast<const uint4 *>(act + (size_t)m0 * K) + i));
+            act_s[i + (i >= K / 8 ? 1 : 0)] = permute8(ld_dependent(reinterpret_cast<const uint4 *>(act + (size_t)m0 * K) + i));
     }
     __syncthreads(); // scales (and staged activations) visible to all warps
     const __half *sA = sc_s + g * G;
@@ -227,7 +227,7 @@ int4_gemv_kernel(const __grid_constant__ CUtensorMap tmW, int M, int N, int K, i
             const float sb = __half2float(sB[si]);
             uint4 av[4];
 #pragma unroll
-            for (int wd = 0; wd < 4; ++wd) av[wd] = kStageAct ? arow_s[kb * 16 + wd] : __ldg(arow + kb * 16 + wd);
+            for (int wd = 0; wd < 4; ++wd) av[wd] = kStageAct ? arow_s[kb * 16 + wd] : ld_dependent(arow + kb * 16 + wd);
             // Two independent accumulator chains halve the mma dependency depth.
             float c0[4], c1[4];
 #pragma unroll
@@ -321,7 +321,7 @@ constexpr int GS_RED = 3;    // partial-sum buffers: a warp is never more than t
 
 template <bool kStageAct>
 __global__ void __launch_bounds__((GS_WARPS + 1) * 32, 2)
-int4_gemv_stream_kernel(const uint8_t *__restrict__ w, int M, int N, int K, int group, const __half *__restrict__ act,
+int4_gemv_stream_kernel(const uint8_t *__restrict__ w, int M, int N, int K, int group, const __half *act,
                         const __half *__restrict__ scales, __half *__restrict__ out, int *status)
 {
     // Shared memory: GS_STAGES x ([16 rows][K/2 B] weights + [16][G] fp16 scales) | GS_RED x [8 warps][16 rows][mrows]
@@ -388,7 +388,7 @@ int4_gemv_stream_kernel(const uint8_t *__restrict__ w, int M, int N, int K, int 
             // 8 consecutive activations -> {k0,k4}, {k1,k5}, {k2,k6}, {k3,k7}: the slot order of the unpacked weights
             const int act_total = mrows * (K / 8);
             for (int i = threadIdx.x; i < act_total; i += GS_WARPS * 32) {
-                const uint4 r = __ldg(reinterpret_cast<const uint4 *>(act) + i);
+                const uint4 r = ld_dependent(reinterpret_cast<const uint4 *>(act) + i);
                 uint4 o;
                 o.x = __byte_perm(r.x, r.z, 0x5410);
                 o.y = __byte_perm(r.x, r.z, 0x7632);
@@ -435,7 +435,7 @@ int4_gemv_stream_kernel(const uint8_t *__restrict__ w, int M, int N, int K, int 
                         av[3] = lds128<48>(aA);
                     } else {
 #pragma unroll
-                        for (int wd = 0; wd < 4; ++wd) av[wd] = __ldg(arow + kb * 16 + wd);
+                        for (int wd = 0; wd < 4; ++wd) av[wd] = ld_dependent(arow + kb * 16 + wd);
                     }
                 }
                 float c0[4], c1[4];

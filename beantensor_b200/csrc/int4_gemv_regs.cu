@@ -33,6 +33,7 @@
 #include <cstring>
 
 #include "btm_internal.h"
+#include "btm_ptx.cuh"
 
 namespace btm {
 
@@ -71,7 +72,7 @@ __device__ __forceinline__ float f16_lo(uint32_t v) { return __half2float(__usho
 __device__ __forceinline__ float f16_hi(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
 
 __global__ void __launch_bounds__(GR_THREADS, 2)
-int4_gemv_regs_kernel(const uint8_t *__restrict__ w, int M, int N, int K, const __half *__restrict__ act,
+int4_gemv_regs_kernel(const uint8_t *__restrict__ w, int M, int N, int K, const __half *act,
                       const __half *__restrict__ scales, __half *__restrict__ out)
 {
     constexpr int NB = GR_NB, W = GR_W;
@@ -130,7 +131,7 @@ int4_gemv_regs_kernel(const uint8_t *__restrict__ w, int M, int N, int K, const 
                 const int i = base0 + u * 32 + lane;
                 const int m = i / PER_WARP, r = i - m * PER_WARP;
                 vv[u] = make_uint4(0u, 0u, 0u, 0u);
-                if (i < total) vv[u] = __ldg(reinterpret_cast<const uint4 *>(act) + (size_t)m * per_row + kb0 * 16 + r);
+                if (i < total) vv[u] = ld_dependent(reinterpret_cast<const uint4 *>(act) + (size_t)m * per_row + kb0 * 16 + r);
             }
 #pragma unroll
             for (int u = 0; u < UN; ++u) {

@@ -99,7 +99,8 @@ struct RawBlock {
     uint32_t w[WORDS];
 };
 
-// vec: 2 = 32-byte loads (the widest there are), 1 = 16-byte, 0 = element by element.
+// Behind griddepcontrol.wait, of what the kernel before may have written (ld_dependent): volatile, or through pointers that
+// nothing promises to be read-only. vec: 2 = 32-byte loads (the widest there are), 1 = 16-byte, 0 = element by element.
 template <typename T>
 __device__ __forceinline__ void load_block(RawBlock<T> &r, const T *p, int vec)
 {
@@ -110,11 +111,12 @@ __device__ __forceinline__ void load_block(RawBlock<T> &r, const T *p, int vec)
             asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                          : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3]), "=r"(r.w[i + 4]), "=r"(r.w[i + 5]), "=r"(r.w[i + 6]),
                            "=r"(r.w[i + 7])
-                         : "l"(reinterpret_cast<const uint32_t *>(p) + i));
+                         : "l"(reinterpret_cast<const uint32_t *>(p) + i)
+                         : "memory");
     } else if (vec == 1) {
 #pragma unroll
         for (int i = 0; i < W; i += 4) {
-            const uint4 q = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i);
+            const uint4 q = ld_dependent(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i));
             r.w[i] = q.x; r.w[i + 1] = q.y; r.w[i + 2] = q.z; r.w[i + 3] = q.w;
         }
     } else if constexpr (sizeof(T) == 4) {
@@ -186,8 +188,8 @@ __device__ __forceinline__ uint32_t encode_block(const RawBlock<T> &r, uint4 &co
 // the issue slots): 16384 x 11008 bf16 in 90 us; so 69.7 us, 6.5 TB/s.
 template <typename T, int kAcross>
 __global__ void __launch_bounds__(mxq::THREADS, sizeof(T) == 4 ? 3 : 4)
-mxfp4_quantize_kernel(const T *__restrict__ x, long long ldx, int vec, int groups, int rows, int K, int steps, const int *offsets,
-                      uint8_t *__restrict__ packed, uint8_t *__restrict__ scales, int *status)
+mxfp4_quantize_kernel(const T *x, long long ldx, int vec, int groups, int rows, int K, int steps, const int *offsets,
+                      uint8_t *packed, uint8_t *scales, int *status)
 {
     using namespace mxq;
     constexpr int BATCH = sizeof(T) == 4 ? 1 : 2, LINES = 64 / kAcross; // rows per pass
@@ -250,8 +252,8 @@ __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { retu
 
 // Bound by memory: 16384 x 11008 to bf16 in 72 us (6.35 TB/s).
 template <typename T>
-__global__ void __launch_bounds__(mxq::THREADS) mxfp4_dequant_kernel(const uint8_t *__restrict__ packed, const uint8_t *__restrict__ scales,
-                                                                     int groups, int rows, int K, const int *offsets, T *__restrict__ out,
+__global__ void __launch_bounds__(mxq::THREADS) mxfp4_dequant_kernel(const uint8_t *packed, const uint8_t *scales,
+                                                                     int groups, int rows, int K, const int *offsets, T *out,
                                                                      long long ldo, int vec, int *status)
 {
     using namespace mxq;
