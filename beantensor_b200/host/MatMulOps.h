@@ -222,32 +222,62 @@ inline void btm_require_mxfp4(const btm_tensor_view &packed, const btm_tensor_vi
     if (packed.gpu_id != scales.gpu_id) throw std::invalid_argument(std::string(name) + ": tensors live on different GPUs");
 }
 
+// The plain side t of a conversion to or from microscaled values beside its packed side: [rows,K], one group or ragged ones by
+// offsets, or the matrices of all experts [groups,N,K], which are dense and have no offsets.
+struct btm_mxfp4_rows {
+    int groups, rows, K;
+    int64_t ld;
+    const int32_t *offsets;
+};
+inline btm_mxfp4_rows btm_require_mxfp4_conversion(const btm_tensor_view &t, const btm_tensor_view &packed, const btm_tensor_view &scales,
+                                                   const btm_tensor_view *offsets, const std::string &name)
+{
+    const int nd = t.ndim == 3 ? 3 : 2;
+    btm_require_gpu_rowmajor(t, nd, name.c_str());
+    if (offsets && nd == 3) throw std::invalid_argument(name + ": offsets go with rank-2 tensors; the groups of a rank-3 one are its first dimension");
+    if (offsets && (offsets->ndim != 1 || offsets->shape[0] == 0)) throw std::invalid_argument(name + ": offsets must be an Int32 tensor of groups + 1 entries");
+    btm_mxfp4_rows r;
+    r.K = btm_dim(t.shape[nd - 1]);
+    uint64_t bytes;
+    if (nd == 3) {
+        r.groups = btm_dim(t.shape[0]);
+        const int N = btm_dim(t.shape[1]);
+        r.rows = btm_dim((uint64_t)r.groups * (uint64_t)N);
+        r.ld = r.K;
+        if ((N > 1 && t.strides[1] != (uint64_t)r.K) || (r.groups > 1 && t.strides[0] != (uint64_t)N * (uint64_t)r.K))
+            throw std::invalid_argument(name + ": a rank-3 tensor must be contiguous");
+        bytes = (uint64_t)r.groups * btm_mxfp4_scale_bytes(1, N, r.K);
+    } else {
+        r.groups = offsets ? btm_dim(offsets->shape[0]) - 1 : 1;
+        r.rows = btm_dim(t.shape[0]);
+        r.ld = btm_pitch(t);
+        bytes = btm_mxfp4_scale_bytes(r.groups, r.rows, r.K);
+    }
+    btm_require_mxfp4(packed, scales, nd, bytes, (name + "(packed)").c_str());
+    bool fits = packed.gpu_id == t.gpu_id && packed.shape[nd - 1] * 2 == t.shape[nd - 1];
+    for (int i = 0; i < nd - 1; ++i) fits = fits && packed.shape[i] == t.shape[i];
+    if (!fits) throw std::invalid_argument(name + ": shape mismatch");
+    r.offsets = offsets ? btm_group_offsets(*offsets, (uint64_t)r.groups, t.gpu_id, (name + "(offsets)").c_str()) : nullptr;
+    return r;
+}
+
 // x [rows,K] (Float32/Float16/BFloat16) -> packed [rows,K/2] and scales; with offsets the scales are laid out for those groups.
+// x [groups,N,K] -> packed [groups,N,K/2] and the scales of one group after the other: the weights of all experts in one call.
 inline void quantize_mxfp4_gpu(const btm_tensor_view &x, btm_tensor_view &packed, btm_tensor_view &scales, const btm_tensor_view *offsets = nullptr,
                                void *stream = nullptr)
 {
-    btm_require_gpu_rowmajor(x, 2, "quantize_mxfp4_gpu(x)");
-    const int groups = offsets ? btm_dim(offsets->shape[0]) - 1 : 1, rows = btm_dim(x.shape[0]), K = btm_dim(x.shape[1]);
-    btm_require_mxfp4(packed, scales, 2, btm_mxfp4_scale_bytes(groups, rows, K), "quantize_mxfp4_gpu(packed)");
-    if (packed.gpu_id != x.gpu_id || packed.shape[0] != x.shape[0] || packed.shape[1] * 2 != x.shape[1])
-        throw std::invalid_argument("quantize_mxfp4_gpu: shape mismatch");
-    const int32_t *offs = offsets ? btm_group_offsets(*offsets, (uint64_t)groups, x.gpu_id, "quantize_mxfp4_gpu(offsets)") : nullptr;
-    btm_raise(btm_mxfp4_quantize(x.gpu_id, stream, x.dtype, groups, rows, K, offs, btm_base(x), btm_pitch(x), const_cast<void *>(btm_base(packed)),
+    const btm_mxfp4_rows r = btm_require_mxfp4_conversion(x, packed, scales, offsets, "quantize_mxfp4_gpu");
+    btm_raise(btm_mxfp4_quantize(x.gpu_id, stream, x.dtype, r.groups, r.rows, r.K, r.offsets, btm_base(x), r.ld, const_cast<void *>(btm_base(packed)),
                                  const_cast<void *>(btm_base(scales))));
 }
 
-// The inverse: out [rows,K] = the values that packed and scales stand for, rounded once to out's dtype.
+// The inverse: out = the values that packed and scales stand for, rounded once to out's dtype; shapes as above.
 inline void dequant_mxfp4_gpu(const btm_tensor_view &packed, const btm_tensor_view &scales, btm_tensor_view &out, const btm_tensor_view *offsets = nullptr,
                               void *stream = nullptr)
 {
-    btm_require_gpu_rowmajor(out, 2, "dequant_mxfp4_gpu(out)");
-    const int groups = offsets ? btm_dim(offsets->shape[0]) - 1 : 1, rows = btm_dim(out.shape[0]), K = btm_dim(out.shape[1]);
-    btm_require_mxfp4(packed, scales, 2, btm_mxfp4_scale_bytes(groups, rows, K), "dequant_mxfp4_gpu(packed)");
-    if (packed.gpu_id != out.gpu_id || packed.shape[0] != out.shape[0] || packed.shape[1] * 2 != out.shape[1])
-        throw std::invalid_argument("dequant_mxfp4_gpu: shape mismatch");
-    const int32_t *offs = offsets ? btm_group_offsets(*offsets, (uint64_t)groups, out.gpu_id, "dequant_mxfp4_gpu(offsets)") : nullptr;
-    btm_raise(btm_mxfp4_dequant(out.gpu_id, stream, out.dtype, groups, rows, K, offs, btm_base(packed), btm_base(scales), const_cast<void *>(btm_base(out)),
-                                btm_pitch(out)));
+    const btm_mxfp4_rows r = btm_require_mxfp4_conversion(out, packed, scales, offsets, "dequant_mxfp4_gpu");
+    btm_raise(btm_mxfp4_dequant(out.gpu_id, stream, out.dtype, r.groups, r.rows, r.K, r.offsets, btm_base(packed), btm_base(scales),
+                                const_cast<void *>(btm_base(out)), r.ld));
 }
 
 // out[M,N] (Float16/BFloat16) = act[M,K] . w[N,K]^T of microscaled operands.
