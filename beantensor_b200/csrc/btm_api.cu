@@ -41,10 +41,12 @@ static std::atomic<int> g_dbg_skip_loads{0};
 static std::atomic<int> g_dbg_bounds{-1};            // -1: not decided yet (BTM_DEBUG_BOUNDS is read once)
 static std::atomic<long long> g_dbg_bounds_shrink{0}; // test hook: pretend C is this many elements shorter
 
-void fill_wait_params(GemmParams *p)
+void fill_wait_params(GemmParams *p, long long depth)
 {
     const long long lim = g_dbg_wait_limit.load(std::memory_order_relaxed);
-    p->wait_limit = lim > 0 ? lim : 2000000000LL; // about one second of SM clocks; the longest kernel here runs milliseconds
+    // About one second of SM clocks, and 64 cycles for every k of the reduction: the epilogue waits for a whole tile, whose
+    // k costs 8 to 16 cycles (512 to 1000 for 64 of them), so that a reduction of some hundred million is no hang.
+    p->wait_limit = (lim > 0 ? lim : 2000000000LL) + 64 * std::max<long long>(p->K, depth);
     p->debug_skip_loads = g_dbg_skip_loads.load(std::memory_order_relaxed);
     int b = g_dbg_bounds.load(std::memory_order_relaxed);
     if (b < 0) {

@@ -60,9 +60,10 @@ struct DeviceState {
 };
 
 int set_error(int code, const char *fmt, ...);
-// Sets p->wait_limit (the default of about one second, or what btm_debug_set installed), the test hooks and, from
-// the fields already set (M, N, batch, ldc, strideC, col0), the extent used by the debug bounds checks.
-void fill_wait_params(GemmParams *p);
+// Sets p->wait_limit (the default of about one second, or what btm_debug_set installed, and an allowance for the depth of the
+// reduction: p->K, or `depth` where that is not it), the test hooks and, from the fields already set (M, N, batch, ldc, strideC,
+// col0), the extent used by the debug bounds checks.
+void fill_wait_params(GemmParams *p, long long depth = 0);
 int check_cuda(cudaError_t e, const char *what);
 DeviceState *device_state(int device); // NULL + error set on failure
 

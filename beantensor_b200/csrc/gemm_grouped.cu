@@ -479,7 +479,7 @@ int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int
     p.strideC = c.strideC;
     p.c_vec_ok = mult16(c.C, c.ldc) && (!c.wgrad || c.groups == 1 || (c.strideC * 2) % 16 == 0) ? 1 : 0;
     p.status = status;
-    fill_wait_params(&p);
+    fill_wait_params(&p, c.wgrad ? c.rows : 0);
     if (p.c_vec_ok) {
         const uint64_t pc = (uint64_t)c.ldc * 2;
         rc = encode_tmap_3d(&tmC, c.dtype, c.C, (uint64_t)c.N, (uint64_t)p.M, (uint64_t)p.batch, pc, p.batch > 1 ? (uint64_t)c.strideC * 2 : pc, 64, 32);

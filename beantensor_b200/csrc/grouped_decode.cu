@@ -379,7 +379,7 @@ static int prepare(DecodeArgs *a, int rows, int groups, int N, int K, const int 
     a->vec = ((uintptr_t)out & 7) == 0 && ldo % 4 == 0;
     GemmParams p;
     memset(&p, 0, sizeof(p));
-    p.M = rows; p.N = N; p.batch = 1; p.ldc = ldo;
+    p.M = rows; p.N = N; p.K = K; p.batch = 1; p.ldc = ldo;
     fill_wait_params(&p);
     a->status = status;
     a->wait_limit = p.wait_limit;

@@ -96,7 +96,7 @@ const char *btm_last_error_string(void);
 
 /* Test hooks, no counterpart in the reference. Process-wide switches that make the bounded waits inside the
  * matmul kernels observable without any fault: "wait_limit_cycles" (SM cycles after which a kernel wait gives
- * up; 0 restores the default of about one second) and "skip_loads" (non-zero: the producer warps of the dense
+ * up, beside 64 for every k of the reduction; 0 restores the default of about one second) and "skip_loads" (non-zero: the producer warps of the dense
  * matmul kernels issue no loads, so the consumers' waits run out, the kernel unwinds, returns, and the next
  * btm_check_device_status reports BTM_ERR_TIMEOUT); "bounds" (non-zero: every store address that a matmul epilogue
  * computes by hand is compared with the extent of C first, a store that would leave it is skipped and reported by
