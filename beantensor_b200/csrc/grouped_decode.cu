@@ -11,8 +11,8 @@
 // Groups are cut into slots of 64 tokens; one with more is read again for each further slot, from L2.
 //
 // Warp roles: 0 weights and tokens by TMA, 1 tcgen05.mma, 2 scales by TMA (microscaled), 4-7 park; all store.
-// A plain product's weights depend on no table: they are asked into L2 before griddepcontrol.wait, under the kernel
-// before (the quantiser of the activations). That is a hint only; they are read after the wait.
+// The weights of a plain product (microscaled only) depend on no table: they are asked into L2 before griddepcontrol.wait,
+// under the kernel before (the quantiser of the activations). That is a hint only; they are read after the wait.
 #include <cstring>
 
 #include <cuda_bf16.h>
@@ -103,14 +103,11 @@ __global__ void __launch_bounds__(dec::THREADS, 2) grouped_decode_kernel(const _
         tmem_alloc<1>(smem_u32(&tmem_base_holder), TMEM_COLS);
         tmem_relinquish<1>();
     }
-    if (warp == 2 && a.offsets == nullptr && elect_one()) {
-        for (int u = u0; u < u1; ++u) {
-            if (KIND == DECODE_KN) {
-                tma_prefetch_3d(&maps.w, n0, u * UNIT_X, 0);
-                if (n0 + 64 < a.N) tma_prefetch_3d(&maps.w, n0 + 64, u * UNIT_X, 0);
-            } else {
+    if constexpr (kMx) { // the 16-bit products always have a table
+        if (warp == 2 && a.offsets == nullptr && elect_one()) {
+            for (int u = u0; u < u1; ++u) {
                 tma_prefetch_3d(&maps.w, u * UNIT_X, n0, 0);
-                if (kMx) tma_prefetch_3d(&maps.sfw, u * 256, n0 / 128, 0);
+                tma_prefetch_3d(&maps.sfw, u * 256, n0 / 128, 0);
             }
         }
     }
