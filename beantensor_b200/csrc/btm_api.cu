@@ -858,7 +858,7 @@ int btm_mxfp4_quantize(int device, void *stream, int src_dtype, int groups, int 
     DeviceState *ds = device_state(device);
     if (!ds) return last_code();
     if (groups == 0 || rows == 0 || K == 0) return BTM_OK;
-    return launch_mxfp4_quantize((cudaStream_t)stream, src_dtype, groups, rows, K, offsets, x, ldx, packed, scales, ds->status);
+    return launch_mxfp4_quantize((cudaStream_t)stream, ds->sm_count, src_dtype, groups, rows, K, offsets, x, ldx, packed, scales, ds->status);
 }
 
 int btm_mxfp4_dequant(int device, void *stream, int dst_dtype, int groups, int rows, int K, const int32_t *offsets, const void *packed,

@@ -130,7 +130,7 @@ int launch_gemm_grouped_pair(const GroupedCall &c, cudaStream_t st, int sm_count
 int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int *status);
 long long grouped_slot_bound(int groups, int rows);
 // Microscaled 4-bit operands (mxfp4.cu). offsets == NULL: every group has rows / groups rows.
-int launch_mxfp4_quantize(cudaStream_t st, int src_dtype, int groups, int rows, int K, const int *offsets, const void *x, long long ldx,
+int launch_mxfp4_quantize(cudaStream_t st, int sm_count, int src_dtype, int groups, int rows, int K, const int *offsets, const void *x, long long ldx,
                           void *packed, void *scales, int *status);
 int launch_mxfp4_dequant(cudaStream_t st, int dst_dtype, int groups, int rows, int K, const int *offsets, const void *packed,
                          const void *scales, void *out, long long ldo, int *status);

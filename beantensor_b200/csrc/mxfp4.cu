@@ -324,15 +324,17 @@ static cudaError_t launch_pdl(void (*kernel)(P...), unsigned grid, cudaStream_t 
 }
 
 template <typename T>
-static int quantize_as(cudaStream_t st, int groups, int rows, int K, const int *offsets, const void *x, long long ldx, void *packed, void *scales, int *status)
+static int quantize_as(cudaStream_t st, int sm_count, int groups, int rows, int K, const int *offsets, const void *x, long long ldx, void *packed, void *scales, int *status)
 {
     const long long slots = slot_count(groups, rows, offsets), chunks = mx_chunks(K);
-    // One block across, 64 rows at a time, while all CTAs are resident at once (four per SM): then the time is a CTA's latency.
+    // One block across, 64 rows at a time, while all CTAs are resident at once (four per SM, 16-bit types): then the time is a CTA's latency.
     // Four across, 16 rows at a time, beyond. Measured, one / four: 256 x 2048 plain (32 CTAs at one) 2.4 / 4.7 us, 3001 x 1440 in 24
     // groups (564) 4.7 / 6.6; 256 x 2048 in 64 groups (1040) 5.1 / 2.8, 2048 x 4096 in 64 (2560) 12.0 / 6.7, 16384 x 11008 71.0 / 69.7.
-    const int across = slots * chunks <= 4 * 148 ? 1 : 4;
+    // The same border serves fp32, of which three CTAs are resident: 2048 x 4096 (512 CTAs at one) 9.8 / 11.0 us.
+    const long long wave = 4LL * sm_count;
+    const int across = slots * chunks <= wave ? 1 : 4;
     // More than one step per CTA once there are several waves of them (four CTAs per SM).
-    long long steps = slots * chunks / (across * 4LL * 4 * 148);
+    long long steps = slots * chunks / (across * 4 * wave);
     steps = steps < 1 ? 1 : steps > 8 ? 8 : steps;
     const long long blocks = slots * ((chunks + steps * across - 1) / (steps * across));
     if (blocks > 0x7FFFFFFFLL) return set_error(BTM_ERR_UNSUPPORTED, "mxfp4 quantise: operand too large (%lld scale blocks)", slots * chunks);
@@ -343,12 +345,12 @@ static int quantize_as(cudaStream_t st, int groups, int rows, int K, const int *
     return check_cuda(e, "mxfp4 quantise launch");
 }
 
-int launch_mxfp4_quantize(cudaStream_t st, int src_dtype, int groups, int rows, int K, const int *offsets, const void *x, long long ldx,
+int launch_mxfp4_quantize(cudaStream_t st, int sm_count, int src_dtype, int groups, int rows, int K, const int *offsets, const void *x, long long ldx,
                           void *packed, void *scales, int *status)
 {
-    if (src_dtype == BTM_F32) return quantize_as<float>(st, groups, rows, K, offsets, x, ldx, packed, scales, status);
-    if (src_dtype == BTM_F16) return quantize_as<__half>(st, groups, rows, K, offsets, x, ldx, packed, scales, status);
-    return quantize_as<__nv_bfloat16>(st, groups, rows, K, offsets, x, ldx, packed, scales, status);
+    if (src_dtype == BTM_F32) return quantize_as<float>(st, sm_count, groups, rows, K, offsets, x, ldx, packed, scales, status);
+    if (src_dtype == BTM_F16) return quantize_as<__half>(st, sm_count, groups, rows, K, offsets, x, ldx, packed, scales, status);
+    return quantize_as<__nv_bfloat16>(st, sm_count, groups, rows, K, offsets, x, ldx, packed, scales, status);
 }
 
 int launch_mxfp4_dequant(cudaStream_t st, int dst_dtype, int groups, int rows, int K, const int *offsets, const void *packed,
