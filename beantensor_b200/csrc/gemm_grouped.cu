@@ -17,12 +17,14 @@
 //              hold rows of the group are multiplied.
 // Few tiles or a ragged last wave: the tile width (256, 128 or 64 columns, and half of it for what would be a partly
 // filled last wave) is chosen on the device from the number of slots, by the same rule in every CTA.
-// Measured (bf16, 16384 rows, 4096 x 4096): product 395 us in one group, 420 in eight (1390, 1310 TFLOP/s), gradient 411;
-// 256 rows in 64 groups of 2048 x 2048 fp16 81 us, 6.6 TB/s. With many rows the tensor core waits for its operands' way: 48 KB per
-// 64-deep k-block at the 73 B per cycle that an SM of a loaded machine gets is 670 cycles, the MMAs take 512.
+// Measured (bf16, 16384 rows, 4096 x 4096, this kernel, after a pause / in a long run under the power cap): product 386 / 457 us in
+// one group, 391 / 468 in eight equal ones, 422 / 502 in eight uneven ones (1430, 1410, 1300 TFLOP/s after a pause), gradient
+// 392 / 472 in eight; 256 rows in 64 groups of 2048 x 2048 fp16 84 us, 6.4 TB/s. With many rows the tensor core waits for its
+// operands' way: 48 KB per 64-deep k-block at the 73 B per cycle that an SM of a loaded machine gets is 670 cycles, the MMAs take 512.
 //
 // General kernel (operands that TMA cannot address, K == 0): 64 x 64 output tiles on CUDA cores as in gemm_simt.cu, fp32
-// accumulation, one rounding. A block finds its group by walking the table.
+// accumulation, one rounding. A block finds its group by walking the table. 4096 rows in eight groups, 1021 x 1023 bf16 in
+// pitches of that width: product 530 us, gradient 485, where 1024 x 1024 take 14 and 15 on the tensor cores.
 #include <cstdlib>
 #include <cstring>
 
@@ -485,10 +487,13 @@ int launch_gemm_grouped(const GroupedCall &c, cudaStream_t st, int sm_count, int
         rc = encode_tmap_3d(&tmC, c.dtype, c.C, (uint64_t)c.N, (uint64_t)p.M, (uint64_t)p.batch, pc, p.batch > 1 ? (uint64_t)c.strideC * 2 : pc, 64, 32);
         if (rc) return rc;
     }
-    // Pairs of CTAs for tall and deep groups. Measured, one CTA against pairs, bf16, rows / N x K:
-    //   16384 in 8 groups / 4096 x 4096: 416 / 408 us    16384 in 16 / 2048 x 4096: 242 / 236    12000 in 4 / 2560 x 2560: 127 / 116
-    //   4096 in 16 / 2048 x 4096: 95.3 / 84.6    8192 in 8 / 1024 x 1024: 23.1 / 22.6    16384 in 64 / 2048 x 2048: 159 / 167
-    //   12000 in 64 / 1024 x 1024: 48.1 / 48.8
+    // Pairs of CTAs for tall and deep groups. Measured, one CTA against pairs, bf16, rows / N x K, us after a pause, equal groups;
+    // uneven ones (a load of rank^-0.7), in which more slots of a pair are cut:
+    //   16384 in 8 groups / 4096 x 4096: 391 / 355; 418 / 379    16384 in 16 / 2048 x 4096: 205 / 186; 230 / 208
+    //   12000 in 4 / 2560 x 2560: 129 / 114; 127 / 113           4096 in 16 / 2048 x 4096: 68.8 / 66.8; 94.1 / 79.2
+    //   8192 in 8 / 1024 x 1024: 24.6 / 22.1; 23.9 / 24.2        16384 in 64 / 2048 x 2048: 128 / 121; 152 / 164
+    //   12000 in 64 / 1024 x 1024: 45.2 / 41.4; 41.6 / 43.2
+    // The table of groups is not known here, so the mean height decides.
     // The weight gradient has no pair form (gemm_grouped_pair.cu).
     const long long height = c.rows / c.groups;
     bool pair = !c.wgrad && height >= 256 && height * c.K > 512 * 1024 && (long long)(c.rows / 256) * ((c.N + 255) / 256) >= sm_count / 4;

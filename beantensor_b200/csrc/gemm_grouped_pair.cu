@@ -1,9 +1,9 @@
 // Two-SM form of the grouped products (gemm_grouped.cu): a tile of a CTA pair is 256 rows x 256 (or 128) columns, one
 // tcgen05.mma.cta_group::2 drives both SMs. Each CTA holds 128 rows of A and half of the columns of B, so a 64-deep
 // k-block costs it 32 KB of loads instead of 48 KB (450 cycles instead of 670 at 73 B per cycle, for 512 of MMAs), and the
-// ring holds half as many k-blocks again. Measured (bf16, 16384 rows, 4096 x 4096): 363 us in eight equal groups (1515 TFLOP/s), 89 %
-// tensor-active; under a long run's power cap 1220 TFLOP/s at 1.31 GHz. Barriers
-// as in gemm_tc2.cu: full[s] lives in the leader and counts the bytes of both CTAs; empty[s] and tmem_full[a] are signalled in
+// ring holds half as many k-blocks again. Measured (bf16, 16384 rows, 4096 x 4096): 355 us in eight equal groups (1550 TFLOP/s) and
+// 379 in eight uneven ones after a pause, 442 and 470 in a long run under the power cap (1250 and 1170 TFLOP/s at 1.2 GHz); 89 %
+// tensor-active. Barriers as in gemm_tc2.cu: full[s] lives in the leader and counts the bytes of both CTAs; empty[s] and tmem_full[a] are signalled in
 // both by multicast tcgen05.commit; tmem_empty[a] lives in the leader and collects the sixteen epilogue warps. No TMA
 // multicast is used.
 //

@@ -352,11 +352,14 @@ static long long slot_bound(int groups, int rows)
 
 // Is this launch one for the decode form? As long as all its tiles are resident at once, two per SM: the split along K then
 // buys parallelism, while further waves would pay this kernel's set-up again and again. Measured, persistent kernel against
-// this one (rows / groups / N x K, tiles):
-//   microscaled  1 / 1 / 11008 x 4096 (86): 11.1 / 6.9 us    64 / 8 / 4096 x 4096 (256): 19.9 / 14.7    1000 / 24 / 1000 x 1440 (312): 10.0 / 9.7
-//                512 / 8 / 4096 x 4096 (480): 21.0 / 24.1    256 / 64 / 2048 x 2048 (1040): 28.7 / 31.6
-//   bf16         2 / 8 / 1024 x 1024 (16): 8.7 / 4.8 us      515 / 16 / 1024 x 512 (184): 9.0 / 6.9      256 / 8 / 4096 x 4096 (352): 46.3 / 44.4
-//                512 / 8 / 4096 x 4096 (480): 47.9 / 58.5    2000 / 40 / 1000 x 1416 (560): 31.7 / 38.5
+// this one (rows / groups / N x K, tiles at most), us in a run, equal groups; uneven ones (a load of rank^-0.7):
+//   microscaled  1 / 1 / 11008 x 4096 (86): 10.2 / 7.7            64 / 8 / 4096 x 4096 (256): 18.2 / 15.6; 18.1 / 15.6
+//                1000 / 24 / 1000 x 1440 (312): 9.2 / 10.8; 10.6 / 11.2   512 / 8 / 4096 x 4096 (480): 19.3 / 18.9; 20.2 / 24.9
+//                256 / 64 / 2048 x 2048 (1040): 30.4 / 35.5; 29.2 / 32.9
+//   bf16         2 / 8 / 1024 x 1024 (16): 8.7 / 5.2              515 / 16 / 1024 x 512 (184): 7.3 / 6.7; 7.3 / 7.7
+//                256 / 8 / 4096 x 4096 (352): 49.5 / 45.2; 49.4 / 46.9    512 / 8 / 4096 x 4096 (480): 51.2 / 48.8; 53.5 / 63.5
+//                2000 / 40 / 1000 x 1416 (560): 31.6 / 37.2; 33.4 / 40.0
+// Just beyond two per SM either may be ahead by some per cent; the border is where the tiles stop being resident.
 bool grouped_decode_fits(int groups, int rows, int N, int sm_count) { return slot_bound(groups, rows) * ((N + dec::BW - 1) / dec::BW) <= 2LL * sm_count; }
 
 // Fills what all kinds share; returns the launch's split and block count.

@@ -185,7 +185,7 @@ __device__ __forceinline__ uint32_t encode_block(const RawBlock<T> &r, uint4 &co
 // after the other, so that a large operand looks its rows up once for several.
 // Bound by memory (2 + 17/32 bytes per value of a 16-bit type). With eight values per thread, the largest magnitude by
 // shuffles and 4-byte stores the kernel was bound by instruction issue (109 instructions per eight values, 79 % of
-// the issue slots): 16384 x 11008 bf16 in 90 us; so 69.7 us, 6.5 TB/s.
+// the issue slots): 16384 x 11008 bf16 in 90 us; so 68 to 71 us, 6.4 to 6.7 TB/s (part of the 96 MB written stays in L2).
 template <typename T, int kAcross>
 __global__ void __launch_bounds__(mxq::THREADS, sizeof(T) == 4 ? 3 : 4)
 mxfp4_quantize_kernel(const T *x, long long ldx, int vec, int groups, int rows, int K, int steps, const int *offsets,

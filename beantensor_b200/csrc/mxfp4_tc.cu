@@ -7,8 +7,8 @@
 // blocks of the weights in one box) and go to tensor memory by one tcgen05.cp per 128 rows x 128 k.
 // One persistent CTA per SM, warp roles and tile walk as in gemm_grouped.cu (a plain product is one group that owns every
 // row), and a second producer warp for the scales: issuing a TMA load takes a thread 75 to 120 cycles, a stage has four
-// to seven, and its MMAs take 384. Measured: 256 rows in 64 groups of 2048 x 2048 27.5 us (5.2 TB/s of weights), 8192 x 11008 x
-// 4096 165 us, where the shared-memory port bounds it (mxfp4_tc_pair.cu).
+// to seven, and its MMAs take 384. Measured: 256 rows in 64 groups of 2048 x 2048 29 us (4.9 TB/s of weights), 8192 x 11008 x
+// 4096 167 us after a pause, 193 in a long run.
 #include <cstdlib>
 #include <cstring>
 
@@ -265,8 +265,9 @@ int launch_mxfp4_matmul(const Mxfp4Call &c, cudaStream_t st, int sm_count, int *
         if (rc) return rc;
     }
     // Pairs of CTAs for tall groups, a deep reduction and enough outputs for their larger tiles. Measured, one CTA against pairs,
-    // rows / N x K:  8192 / 11008 x 4096: 165 / 159 us    2048 / 4096 x 4096: 23.7 / 21.2    4096 in 8 groups / 4096 x 4096: 43.7 / 42.0
-    //   1024 / 4096 x 4096: 13.8 / 15.5    8192 / 2048 x 1024: 14.6 / 17.7    12000 in 24 groups / 4096 x 2048: 65.9 / 67.4
+    // rows / N x K, us in a run, equal groups; uneven ones (a load of rank^-0.7):
+    //   8192 / 11008 x 4096: 193 / 188    2048 / 4096 x 4096: 26.7 / 23.3    4096 in 8 groups / 4096 x 4096: 47.1 / 44.1; 51.3 / 54.4
+    //   1024 / 4096 x 4096: 15.9 / 15.7   8192 / 2048 x 1024: 15.9 / 18.4    12000 in 24 / 4096 x 2048: 76.9 / 70.8; 77.5 / 78.3
     bool pair = c.rows / c.groups >= 512 && c.K >= 2048 && (long long)c.rows * c.N >= 8 << 20;
     if (force) {
         if (!strcmp(force, "1cta")) pair = false;

@@ -1,9 +1,9 @@
 // Two-SM form of the microscaled product (mxfp4_tc.cu): a tile of a CTA pair is 256 rows x 192 (or 128) columns, each CTA
 // holds 128 rows of the activations and half of the weight rows, so a 256-deep stage costs it 31 KB of loads instead of 43.
-// What bounds it is the shared-memory port: per stage the tensor core reads 16 KB of A and 24 KB of B, 31 KB arrive, 3 KB of
-// scales leave for tensor memory and the epilogue moves 6 KB, together 625 cycles at 128 B per cycle; measured 620, where the
-// MMAs take 384. 8192 x 11008 x 4096: 154 to 160 us (4.7 PFLOP/s). Measured without effect: the scale copies in a warp of their
-// own, no tile look-up in the MMA issuer.
+// 8192 x 11008 x 4096: 162 us after a pause (4.6 PFLOP/s), 188 in a long run under the power cap. That is 620 to 630 cycles a stage,
+// where the MMAs take 384 and 31 KB of loads at the 73 B per cycle of a loaded machine 435. Which wait makes up the rest is not
+// known: no unit is above 67 % (tensor pipe 59 %, its path to memory 60 %, data banks of shared memory 20 % each for reads and
+// writes). Measured without effect: the scale copies in a warp of their own, no tile look-up in the MMA issuer.
 //
 // Every load, scales included, is a tensor-map load whose completion goes to the leader's full[s]; the scale blocks are
 // one matrix of 32-bit words (a row block per row), so that both row blocks of the weights come in one box. Issuing a TMA load

@@ -208,10 +208,11 @@ int btm_bmm(int device, void *stream, int dtype, int batch, int M, int N, int K,
  * per-device pool and multiplied by the dense tensor-core kernel, instead of being unpacked again
  * for every 128 rows). K % group == 0, group % 32 == 0, K % 32 == 0.
  * Ordering: the products use programmatic dependent launch. If the preceding kernel on the
- * stream is another int4 product of this library, this one may read w_packed and scales_f16 while
- * that kernel is still running (act_f16 is read and out_f16 written only after it has completed);
- * w_packed and scales_f16 must therefore not be the output of an immediately preceding int4 product, nor of a
- * grouped or microscaled call (below), which let their successor in early too. */
+ * stream is one that lets its successor in early (any product of this library, a microscaled conversion), this one
+ * may read w_packed and scales_f16 while that kernel, and a chain of such kernels in front of it, is still running
+ * (act_f16 is read and out_f16 written only after they have completed). So w_packed and scales_f16 must not be the
+ * output of such a call unless something that lets no successor in early lies between: btm_int4_quantize, btm_convert, a
+ * copy, a kernel of somebody else's, a synchronisation. What btm_int4_quantize writes is always safe. */
 int btm_int4_matmul(int device, void *stream, int M, int N, int K, int group, const void *act_f16,
                     const void *w_packed, const void *scales_f16, void *out_f16);
 
@@ -245,8 +246,8 @@ int btm_int4_unpack(int device, void *stream, int N, int K, const void *w_packed
  * it extends Ops/Algebra/MatMul as btm_bmm does, to batches of unequal height.
  *   offsets  device memory, groups + 1 values, not decreasing, within [0, rows]; read by the kernel in stream order, so
  *            it may be the output of work queued before. rows = rows of A and C. Rows in front of offsets[0] and behind
- *            offsets[groups] belong to no group: they are not read and C keeps what it held there. A group may be
- *            empty. Entries that break these rules never lead outside the operands: they are clamped to [0, rows], an
+ *            offsets[groups] belong to no group: whatever A holds there has no effect (a tile may load up to 63 rows
+ *            behind its group, within A), and C keeps what it held there. A group may be empty. Entries that break these rules never lead outside the operands: they are clamped to [0, rows], an
  *            entry smaller than an earlier one counts as that earlier one, and the next btm_check_device_status
  *            returns BTM_ERR_INVALID.
  * dtype BTM_F16 or BTM_BF16, fp32 accumulation, one rounding. lda >= K, ldc >= N. Alignment as btm_gemm: operands that
