@@ -19,6 +19,19 @@ from .errors import GPUTaskOnCPUBuild, raise_for_status
 _DT = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
 
 
+# A call into the library makes its device current on the calling thread; the functions here put back the one that was. With one
+# GPU there is nothing to put back, and looking it up takes 0.2 us of a call's 6.5: the first call counts them.
+_ONE_GPU = _counted = False
+_set_device = torch._C._cuda_setDevice
+
+
+def _current_device() -> int:
+    global _ONE_GPU, _counted
+    if not _counted:
+        _counted, _ONE_GPU = True, torch.cuda.device_count() == 1
+    return torch._C._cuda_getDevice()
+
+
 def _LIB():
     return _lib._lib or _lib.lib()
 
@@ -52,7 +65,11 @@ def init(device: int = 0) -> None:
 
 
 def check_device_status(device: int = 0) -> None:
-    raise_for_status(_lib.lib().btm_check_device_status(device, _stream(device)))
+    cur = device if _ONE_GPU else _current_device()
+    rc = _lib.lib().btm_check_device_status(device, _stream(device))
+    if cur != device:
+        _set_device(cur)
+    raise_for_status(rc)
 
 
 def matmul_gpu(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor, bias: torch.Tensor | None = None,
@@ -86,12 +103,16 @@ def matmul_gpu(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor, bias: torch.
         # Transposed or strided views (Tensor::strides, Tensor/Tensor.h:173-195) go through without a copy.
         if bias is not None or relu:
             raise ValueError("matmul_gpu: the fused epilogue takes row-major operands")
+        cur = dev if _ONE_GPU else _current_device()
         rc = _LIB().btm_gemm_strided(dev, _stream(dev), _DT[a.dtype], M, N, K, a.data_ptr(), a.stride(0), a.stride(1),
                                      b.data_ptr(), b.stride(0), b.stride(1), out.data_ptr(), ldc)
+        if cur != dev:
+            _set_device(cur)
         raise_for_status(rc)
         return
     lda = a.stride(0) if M > 1 else max(K, 1)
     ldb = b.stride(0) if K > 1 else max(N, 1)
+    cur = dev if _ONE_GPU else _current_device()
     if bias is None and not relu:
         rc = _lib.lib().btm_gemm(dev, _stream(dev), _DT[a.dtype], M, N, K, a.data_ptr(), lda, b.data_ptr(), ldb,
                                  out.data_ptr(), ldc)
@@ -99,6 +120,8 @@ def matmul_gpu(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor, bias: torch.
         rc = _lib.lib().btm_gemm_bias_act(dev, _stream(dev), _DT[a.dtype], M, N, K, a.data_ptr(), lda, b.data_ptr(), ldb,
                                           bias.data_ptr() if bias is not None else None, 1 if relu else 0,
                                           out.data_ptr(), ldc)
+    if cur != dev:
+        _set_device(cur)
     raise_for_status(rc)
 
 
@@ -122,8 +145,11 @@ def bmm_gpu(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor) -> None:
     sa = a.stride(0) if B > 1 else M * K
     sb = b.stride(0) if B > 1 else K * N
     sc = out.stride(0) if B > 1 else M * N
+    cur = dev if _ONE_GPU else _current_device()
     rc = _lib.lib().btm_bmm(dev, _stream(dev), _DT[a.dtype], B, M, N, K, a.data_ptr(), sa, b.data_ptr(), sb,
                             out.data_ptr(), sc)
+    if cur != dev:
+        _set_device(cur)
     raise_for_status(rc)
 
 
@@ -148,8 +174,11 @@ def matmul_int4_gpu(act: torch.Tensor, w_packed: torch.Tensor, scales: torch.Ten
         raise ValueError("matmul_int4_gpu: shape mismatch")
     if not (act.is_contiguous() and w_packed.is_contiguous() and scales.is_contiguous() and out.is_contiguous()):
         raise ValueError("matmul_int4_gpu: tensors must be contiguous")
+    cur = dev if _ONE_GPU else _current_device()
     rc = _LIB().btm_int4_matmul(dev, torch._C._cuda_getCurrentRawStream(dev), M, N, K, group, act.data_ptr(), w_packed.data_ptr(),
                                 scales.data_ptr(), out.data_ptr())
+    if cur != dev:
+        _set_device(cur)
     if rc:
         raise_for_status(rc)
 
@@ -160,7 +189,10 @@ def dequant_int4_gpu(w_packed: torch.Tensor, scales: torch.Tensor, out: torch.Te
     K = K2 * 2
     if out.shape != (N, K) or out.dtype != torch.float16 or scales.dtype != torch.float16:
         raise ValueError("dequant_int4_gpu: shape or dtype mismatch")
+    cur = dev if _ONE_GPU else _current_device()
     rc = _lib.lib().btm_int4_dequant(dev, _stream(dev), N, K, group, w_packed.data_ptr(), scales.data_ptr(), out.data_ptr())
+    if cur != dev:
+        _set_device(cur)
     raise_for_status(rc)
 
 
@@ -169,7 +201,10 @@ def unpack_int4_gpu(w_packed: torch.Tensor, out: torch.Tensor) -> None:
     N, K2 = w_packed.shape
     if out.shape != (N, K2 * 2) or out.dtype != torch.int8:
         raise ValueError("unpack_int4_gpu: shape or dtype mismatch")
+    cur = dev if _ONE_GPU else _current_device()
     rc = _lib.lib().btm_int4_unpack(dev, _stream(dev), N, K2 * 2, w_packed.data_ptr(), out.data_ptr())
+    if cur != dev:
+        _set_device(cur)
     raise_for_status(rc)
 
 
@@ -184,7 +219,10 @@ def quantize_int4_gpu(w: torch.Tensor, w_packed: torch.Tensor, scales: torch.Ten
     for t in (w, w_packed, scales):
         if not t.is_contiguous():
             raise ValueError("quantize_int4_gpu: tensors must be contiguous")
+    cur = dev if _ONE_GPU else _current_device()
     rc = _lib.lib().btm_int4_quantize(dev, _stream(dev), N, K, group, w.data_ptr(), w_packed.data_ptr(), scales.data_ptr())
+    if cur != dev:
+        _set_device(cur)
     raise_for_status(rc)
 
 
@@ -259,8 +297,11 @@ def grouped_matmul_gpu(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor, 
         ldb, outer = (bn if N > 1 else K or 1), N
     else:
         raise ValueError("grouped_matmul_gpu: each matrix of b must be row-major or transposed row-major")
+    cur = dev if _ONE_GPU else _current_device()
     rc = _LIB().btm_gemm_grouped(dev, _raw_stream(dev), dt, G, rows, N, K, offsets.data_ptr(), a.data_ptr(), lda, b.data_ptr(),
                                  bg if G > 1 else outer * ldb, ldb, 1 if trans else 0, out.data_ptr(), ldc)
+    if cur != dev:
+        _set_device(cur)
     if rc:
         raise_for_status(rc)
 
@@ -291,8 +332,11 @@ def grouped_matmul_wgrad_gpu(a: torch.Tensor, dout: torch.Tensor, offsets: torch
     if (rows | N | K | G) >> 31:
         _too_large("grouped_matmul_wgrad_gpu")
     lda, ldd, ldc = _row_pitch(a, rows, K, "a"), _row_pitch(dout, rows, N, "dout"), _row_pitch(out, K, N, "out")
+    cur = dev if _ONE_GPU else _current_device()
     rc = _LIB().btm_gemm_grouped_wgrad(dev, _raw_stream(dev), dt, G, rows, K, N, offsets.data_ptr(), a.data_ptr(), lda, dout.data_ptr(), ldd,
                                        out.data_ptr(), out.stride(0) if G > 1 else K * ldc, ldc)
+    if cur != dev:
+        _set_device(cur)
     if rc:
         raise_for_status(rc)
 
@@ -349,10 +393,13 @@ def _mxfp4_convert(fn, x: torch.Tensor, packed: torch.Tensor, scales: torch.Tens
         _bad_mxfp4(packed, scales, K, what, fits)
     if (rows | K | groups) >> 31:
         _too_large(what)
+    cur = dev if _ONE_GPU else _current_device()
     if quantize:
         rc = fn(dev, _raw_stream(dev), dt, groups, rows, K, table, x.data_ptr(), ld, packed.data_ptr(), scales.data_ptr())
     else:
         rc = fn(dev, _raw_stream(dev), dt, groups, rows, K, table, packed.data_ptr(), scales.data_ptr(), x.data_ptr(), ld)
+    if cur != dev:
+        _set_device(cur)
     if rc:
         raise_for_status(rc)
 
@@ -399,8 +446,11 @@ def matmul_mxfp4_gpu(act: torch.Tensor, act_scales: torch.Tensor, w: torch.Tenso
     if (M | N | K) >> 31:
         _too_large("matmul_mxfp4_gpu")
     dt = _mxfp4_product_dtype("matmul_mxfp4_gpu", act, act_scales, w, w_scales, out, K)
+    cur = dev if _ONE_GPU else _current_device()
     rc = _LIB().btm_mxfp4_matmul(dev, _raw_stream(dev), dt, M, N, K, act.data_ptr(), act_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(),
                                  out.data_ptr(), _row_pitch(out, M, N, "out"))
+    if cur != dev:
+        _set_device(cur)
     if rc:
         raise_for_status(rc)
 
@@ -425,8 +475,11 @@ def grouped_matmul_mxfp4_gpu(act: torch.Tensor, act_scales: torch.Tensor, w: tor
     if (rows | N | K | G) >> 31:
         _too_large("grouped_matmul_mxfp4_gpu")
     dt = _mxfp4_product_dtype("grouped_matmul_mxfp4_gpu", act, act_scales, w, w_scales, out, K)
+    cur = dev if _ONE_GPU else _current_device()
     rc = _LIB().btm_mxfp4_matmul_grouped(dev, _raw_stream(dev), dt, G, rows, N, K, offsets.data_ptr(), act.data_ptr(), act_scales.data_ptr(),
                                          w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), _row_pitch(out, rows, N, "out"))
+    if cur != dev:
+        _set_device(cur)
     if rc:
         raise_for_status(rc)
 
@@ -440,7 +493,10 @@ def convert_gpu(src: torch.Tensor, dst: torch.Tensor) -> None:
     if src.dtype not in _DT or dst.dtype not in _DT:
         from .errors import NotImplementedOp
         raise NotImplementedOp(f"convert_gpu: {src.dtype} -> {dst.dtype} is not supported")
+    cur = dev if _ONE_GPU else _current_device()
     rc = _lib.lib().btm_convert(dev, _stream(dev), _DT[src.dtype], _DT[dst.dtype], src.numel(), src.data_ptr(), dst.data_ptr())
+    if cur != dev:
+        _set_device(cur)
     raise_for_status(rc)
 
 
