@@ -3,8 +3,8 @@
 // Some hosts of this library cannot call cudaMalloc at the moment they need a product: a
 // thread-pool worker that runs while another thread holds the allocator, code that has handed
 // all device memory to its own pool at start-up, or a service whose memory budget is fixed once
-// and audited. The ordinary fp32 entry point keeps a per-device scratch buffer and grows it with
-// cudaMalloc when a larger shape arrives, so it is not usable there. This variant runs the same
+// and audited. The ordinary fp32 entry point takes its scratch from a memory pool, which asks the
+// driver for more when a larger shape arrives, so it is not usable there. This variant runs the same
 // kernels with the scratch (the hi/lo operand planes) in a fixed array that is part of the
 // library image: nothing is allocated or freed, on any call.
 //

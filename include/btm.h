@@ -128,7 +128,8 @@ int btm_check_device_status(int device, void *stream);
  *   (cudaMallocFromPoolAsync / cudaFreeAsync), so concurrent calls on other streams or threads never
  *   share scratch; freed blocks stay in the pool, and only the first call of a larger shape reaches
  *   the driver. Infinite inputs give infinite (not NaN) outputs, as a plain fp32 product would.
- * lda >= K, ldb >= N, ldc >= N, in elements. Any M, N, K >= 0; shapes or pointers that
+ * lda >= K, ldb >= N, ldc >= N, in elements; what C holds between column N and ldc is kept, here and in every other
+ * call with an output pitch. Any M, N, K >= 0; shapes or pointers that
  * the tensor-core path cannot address (row pitch or base not 16-byte aligned) run on a
  * general CUDA-core kernel with the same arithmetic contract. */
 int btm_gemm(int device, void *stream, int dtype, int M, int N, int K, const void *A, int64_t lda, const void *B,
